@@ -231,8 +231,8 @@ __device__ __forceinline__ float gelu_new_r(float x) {
 }
 
 // gelu_new on TWO elements at once, same rounding points as gelu_new_r: the seven intermediate roundings go through one
-// packed convert each (v_cvt_pk_*: half the converts of the scalar form), the arithmetic through packed fp32
-// instructions where the compiler finds them; the LAST rounding is left to the caller's pack2 (rounding twice is the
+// packed convert each (v_cvt_pk_*: half the converts of the scalar form), the arithmetic on 2-element
+// vectors; the LAST rounding is left to the caller's pack2 (rounding twice is the
 // identity).  exp(2u) = exp2(u * 2 log2(e)): the same product as __expf(2u) (scaling by 2 commutes with rounding).
 template <int DT>
 __device__ __forceinline__ void gelu_new_pair(float &a, float &b) {

@@ -260,9 +260,9 @@ __global__ __launch_bounds__(GATE_STREAM_THREADS) void gate_logits_stream_kernel
     __syncthreads();
     if (!has0) return;  // (after the only barrier)
     auto compute_pair = [&](int pr, const uint4 (&q)[NSL][R]) {
-        // the FMAs go two at a time through v_pk_fma_f32 (two independent IEEE FMAs: the chains are unchanged): the two
-        // rows of the pair with one wg value (R = 2), or two experts with one x value (R = 1).  As scalar v_fmac_f32 they
-        // were ~1000 of the ~1750 VALU cycles a wave spends per row pair.
+        // the FMAs are written two at a time (two independent IEEE FMAs: the chains are unchanged): the two
+        // rows of the pair with one wg value (R = 2), or two experts with one x value (R = 1).  The build keeps packed
+        // fp32 instructions off, so they run as scalar FMAs (~1000 of the ~1750 VALU cycles a wave spends per row pair).
         typedef float f32x2_t __attribute__((ext_vector_type(2)));
         constexpr int NP = R * EMAX / 2;  // packed accumulators: [e] = rows (0, 1) when R == 2, [e / 2] = experts (e, e + 1) when R == 1
         static_assert(R == 1 || R == 2, "rows per step");
