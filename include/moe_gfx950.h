@@ -356,6 +356,62 @@ int moe_dispatch_bwd(const void *da_rows, const int32_t *expert_idx, const int32
                      const float *dlogits, const void *wg, int wg_is_bf16, int S, int M, int E, int top_k, void *dx,
                      uint64_t jitter_seed, void *stream);
 
+/* ---- 8-bit experts: norm, products, expert MLP --------------------------------------------------------------
+ * No counterpart in the reference, whose experts run in 16 bits.  Format: e4m3 (OCP) elements; one power-of-two scale 2^e
+ * per 1 x 128 block of a row and per 128 x 128 block of a weight matrix, held as an e8m0 byte e + 127, e the smallest with
+ * max|block| * 2^-e <= 448 (scaling rounds nothing).  A block that holds an infinity or a NaN becomes NaN (byte 255), and so
+ * does every product that reads it.  The last block of a row, and of a matrix in either direction, may be short.
+ * Row scales: [rows, ceil(K/128)] with a row stride that is a multiple of 4 bytes, 4-byte aligned, the padding readable;
+ * weight scales: dense [experts, ceil(N/128), ceil(K/128)], for the gated W1 [experts, 2 * ceil(I/128), ceil(M/128)] (each
+ * projection has a grid of its own). */
+
+/* moe_add_rms_norm_fwd: sum = round(x + residual); y = sum * weight / sqrt(mean(sum^2) + eps) in fp32, rounded once.
+ *   x, residual [S,M] of type dtype with row strides ldx, ldr (any; wide loads where strides, M and pointers allow them);
+ *   residual NULL: sum = x, and the sum output may be NULL
+ *   weight [M] fp32 (MOE_WG_F32) or of the rows' type (MOE_WG_BF16 / MOE_WG_F16)
+ *   y [S,M] or NULL; sum [S,M]; rstd [S] fp32 or NULL (kept for the backward pass)
+ *   q, scale: e4m3 rows of the UNROUNDED y, both or neither; M % 16 == 0, ldq % 8 == 0 then.  1 <= M <= 65536.  One launch.
+ * moe_add_rms_norm_bwd: dx (gradient of x and of residual) and dweight (in the weight's type) from dy and dsum (either may
+ * be NULL = 0), the kept sum and rstd.  Two launches, fixed summation order. */
+int moe_add_rms_norm_fwd(const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight, int w_dtype,
+                         float eps, int S, int M, void *y, int64_t ldy, void *sum, int64_t lds, float *rstd, void *q,
+                         int64_t ldq, void *scale, int64_t ld_scale, int dtype, void *stream);
+size_t moe_add_rms_norm_bwd_workspace_bytes(int S, int M);
+int moe_add_rms_norm_bwd(const void *dy, int64_t lddy, const void *dsum, int64_t ldds, const void *sum, int64_t lds,
+                         const void *weight, int w_dtype, const float *rstd, int S, int M, void *dx, int64_t lddx,
+                         void *dweight, void *workspace, size_t ws_bytes, int dtype, void *stream);
+
+/* moe_quantize_rows_fp8: 16-bit rows [S,M] -> e4m3 rows + scales.  moe_quantize_blocks_fp8: dense 16-bit weights
+ * [batch, n, k] -> e4m3 + scales (a gated W1 [E, 2I, M] is quantised as batch = 2E, n = I).  moe_transpose_blocks_fp8:
+ * [batch, n, k] -> [batch, k, n] with its scales, for the input gradient.  M, k % 16 == 0 (transpose: n too). */
+int moe_quantize_rows_fp8(const void *x, int64_t ldx, int S, int M, void *q, int64_t ldq, void *scale, int64_t ld_scale,
+                          int dtype, void *stream);
+int moe_quantize_blocks_fp8(const void *w, int batch, int n, int k, void *q, void *scale, int dtype, void *stream);
+int moe_transpose_blocks_fp8(const void *w, const void *scale, int batch, int n, int k, void *wt, void *scale_t, void *stream);
+
+/* moe_grouped_gemm_fp8_fwd: moe_grouped_gemm_fwd (plain epilogue) on 8-bit operands, fp32 accumulation.
+ *   a e4m3 rows (stride lda bytes, % 16), gather / gather_shift / group_offsets / G / max_rows as there; group_offsets NULL
+ *   with G = 1: all max_rows rows use expert 0
+ *   w [n_experts_local, N, K] e4m3 dense, bias [n_experts_local, N] of type dtype or NULL, out [*, N] of type dtype
+ *   zero_tail: rows of out in [0, max_rows) outside [group_offsets[0], group_offsets[G]) are set to 0 (else untouched)
+ * 16 <= K <= 65536, K % 16 == 0, any N.  One launch. */
+int moe_grouped_gemm_fp8_fwd(const void *a, int64_t lda, const void *a_scale, int64_t ld_as, const int32_t *gather,
+                             int gather_shift, const void *w, const void *w_scale, const void *bias,
+                             const int32_t *group_offsets, int G, int n_experts_local, int max_rows, int K, int N,
+                             int zero_tail, void *out, int64_t ldo, int dtype, void *stream);
+
+/* moe_expert_ffn_fp8_fwd: moe_expert_ffn_fwd on 8-bit experts.  Activation in fp32 on the accumulators (no 16-bit rounding
+ * between the products), quantised per 1 x 128 block of the I hidden channels for the second product.
+ *   x [src_rows, M] 16-bit rows (quantised into the workspace), or NULL and a / a_scale: rows that are 8-bit already
+ *   workspace of moe_expert_ffn_fp8_workspace_bytes(x ? src_rows : 0, max_rows, M, I) bytes, contents meaningless between
+ *   calls; calls that may overlap need one each.  M % 16 == 0, I % 16 == 0.  Fixed launch count. */
+size_t moe_expert_ffn_fp8_workspace_bytes(int src_rows, int max_rows, int M, int I);
+int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int src_rows, const void *a, int64_t lda, const void *a_scale,
+                           int64_t ld_as, const int32_t *gather, int gather_shift, const void *w1, const void *w1_scale,
+                           const void *b1, const void *w2, const void *w2_scale, const void *b2,
+                           const int32_t *group_offsets, int G, int n_experts_local, int max_rows, int M, int I,
+                           int n_gated, void *workspace, size_t ws_bytes, void *y, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 # MOE_GFX950_LIB points the loader at another build of the same ABI (kernel A/B experiments, tools/variants)
@@ -76,6 +76,30 @@ _SIGNATURES = [
     ("moe_dispatch_bwd", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
       c_uint64, c_void_p]),
+    # ---- 8-bit experts ----
+    ("moe_add_rms_norm_fwd", c_int,
+     [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_float, c_int, c_int, c_void_p, c_int64, c_void_p,
+      c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),
+    ("moe_add_rms_norm_bwd_workspace_bytes", c_size_t,
+     [c_int, c_int]),
+    ("moe_add_rms_norm_bwd", c_int,
+     [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+      c_int64, c_void_p, c_void_p, c_size_t, c_int, c_void_p]),
+    ("moe_quantize_rows_fp8", c_int,
+     [c_void_p, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),
+    ("moe_quantize_blocks_fp8", c_int,
+     [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    ("moe_transpose_blocks_fp8", c_int,
+     [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    ("moe_grouped_gemm_fp8_fwd", c_int,
+     [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+      c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p]),
+    ("moe_expert_ffn_fp8_workspace_bytes", c_size_t,
+     [c_int, c_int, c_int, c_int]),
+    ("moe_expert_ffn_fp8_fwd", c_int,
+     [c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p,
+      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t,
+      c_void_p, c_int, c_void_p]),
 ]
 
 class BlockTop2Args(ctypes.Structure):

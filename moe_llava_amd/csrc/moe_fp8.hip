@@ -1,0 +1,590 @@
+// Grouped, variable-length matrix products in 8 bits on MFMA for gfx950: e4m3 operands with a power-of-two scale for every
+// 1 x 128 block of the rows and every 128 x 128 block of the weights (moe_fp8.h).
+//
+//   out[r, n] = sum_b 2^(ea[r, b] + ew[n / 128, b]) * sum_{k in block b} qa[r, k] * qw[n, k]   (+ bias)     fp32 accumulation
+//
+// plain (16-bit output), or as the first product of an expert MLP: SwiGLU / gelu_new in fp32 on the accumulators, and the
+// result quantised again for the second product (the activation never leaves the kernel in more than 8 bits).
+//
+// Tile BM (rows) x BNW (weight rows) x 128 (K) per 512-thread block, 8 waves as 2 (rows) x 4 (weight rows).  One ring slot
+// is one K slice = one block of the scales, so v_mfma_scale_f32_16x16x128_f8f6f4 takes the two exponent bytes of the slice
+// as operands and accumulates in place: no vector instruction per block of K.  A slice is 128 bytes of every operand row,
+// the geometry of the 16-bit tile (moe_gemm.hip: LDS-DMA fills, XOR swizzle on the source address and on the read, loader
+// waves 0-3), at twice the multiplications per byte.  Lane (fr, fq) of a fragment holds the 16-byte chunks fq and fq + 4 of
+// its row: any split of the 128 columns over the lanes is right as long as both operands use the same one.
+// The scale bytes of a whole tile (rows x K / 128, and two rows of the weights' grid) are put in LDS once per tile by the
+// waves that do not load operands.
+#include "moe_fp8.h"
+
+namespace moe {
+
+typedef __attribute__((ext_vector_type(8))) int v8i_t;
+typedef __attribute__((ext_vector_type(4))) int v4i_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef unsigned char u8;
+
+struct Fp8GemmParams {
+    const u8 *a;              // rows, e4m3, row stride lda bytes
+    long long lda;
+    const u8 *a_scale;        // e8m0 [rows, ceil(K/128)], row stride lds_a bytes (a multiple of 4, rows 4-byte aligned)
+    long long ld_as;
+    const int *gather;
+    int gather_shift;
+    const u8 *w;              // [experts, N (or 2N), K]
+    long long w_expert_stride;
+    const u8 *w_scale;        // [experts, blocks of N (or 2x), ceil(K/128)], dense
+    long long ws_expert_stride;
+    const bf16_t *bias;
+    long long bias_expert_stride;
+    const int *group_offsets; // NULL: one group, rows [0, max_rows)
+    int G, n_experts, max_rows;
+    void *out;                // 16-bit [rows, ldo], or e4m3 with out_scale
+    long long ldo;
+    u8 *out_scale;            // [rows, ceil(N/128)], row stride ld_os
+    long long ld_os;
+    int K, N_out;
+    int b_row_offset;         // gated: weight row of the first 'b' projection row (= N_out)
+    int b_blk_offset;         // gated: row of the scales' grid where the 'b' projection starts
+    int n_gated;
+    int col_tiles, rs;
+    int vec_store;            // 16-bit output: rows and pointer allow 16-byte stores
+    int zero_tail;            // 16-bit output: rows of [0, max_rows) that belong to no group are set to 0
+};
+
+constexpr int FTHREADS = 512;
+constexpr int FLW = 4;                 // loader waves (one per SIMD)
+constexpr int FP8_STRIP = 28672;       // LDS bytes for the rows' scales of a tile
+constexpr int FP8_WS_ROW = 512;        // ... and for each of the two rows of the weights' scales: K <= 65536
+constexpr int FP8_MAX_K = FP8_WS_ROW * QB;
+
+__device__ const uint4 g_fp8_zero = {0u, 0u, 0u, 0u};  // source of the columns behind K in the last slice
+
+__device__ __forceinline__ void glds16b(const u8 *gsrc, char *lds_wave_base) {
+    __builtin_amdgcn_global_load_lds(
+        reinterpret_cast<const __attribute__((address_space(1))) void *>(reinterpret_cast<uintptr_t>(gsrc)),
+        reinterpret_cast<__attribute__((address_space(3))) void *>(
+            static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds_wave_base))),
+        16, 0, 0);
+}
+template <int N>
+__device__ __forceinline__ void fwait_vm_barrier() {
+    // all but the N youngest of this wave's fills have landed, then everybody's have (a __syncthreads would drain them all)
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+template <int N>
+struct FInt { static constexpr int value = N; };
+
+template <int EPI, int BM, int BNW>
+struct FTile {
+    static constexpr bool GATED = EPI == EPI_SWIGLU;
+    static constexpr bool QOUT = EPI != EPI_PLAIN;            // output quantised for the next product
+    static_assert(BM == 256 || BM == 128 || BM == 64 || BM == 32, "row tile");
+    static_assert(BNW == 256 || ((BNW == 128 || BNW == 64) && !GATED), "column tile");
+    static_assert(!QOUT || (GATED ? BNW / 2 : BNW) % QB == 0, "an output block lies in one tile");
+    static constexpr int SLOT = (BM + BNW) * QB;              // bytes of one K slice
+    static constexpr int NS = (131072 / SLOT) > 8 ? 8 : (131072 / SLOT);
+    static constexpr int NC = GATED ? BNW / 2 : BNW;          // output columns
+    static constexpr int ROWB = (QOUT ? NC : NC * 2) + 16;    // bytes of an image row
+    static constexpr int XS = NS * SLOT;                      // offset of the rows' scales
+    static constexpr int WS = XS + FP8_STRIP;                 // ... of the weights' scales
+    static constexpr int TOP = BM * ROWB;                     // offset of the block maxima (epilogue): [4][BM]
+    static constexpr int LDS_K = WS + 2 * FP8_WS_ROW;
+    static constexpr int LDS_E = TOP + (QOUT ? 4 * BM * 4 : 0);
+    static constexpr int LDS_BYTES = LDS_K > LDS_E ? LDS_K : LDS_E;
+    static_assert(NS >= 2 && LDS_BYTES <= 163840, "LDS");
+    static constexpr int NF = BNW / 64;                       // 16-row weight fragments per wave
+    static constexpr int WNT = BNW / 4;                       // weight rows per wave
+};
+
+// activations in fp32 (nothing is rounded between the accumulator and the quantisation: a 16-bit rounding there would move
+// ~1 % of the elements to a neighbouring e4m3 value)
+__device__ __forceinline__ float gelu_new_f32(float x) {
+    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
+    // 0.5 x (1 + tanh u) = x / (1 + exp(-2u))
+    return x * __builtin_amdgcn_rcpf(1.f + __expf(-2.f * u));
+}
+
+template <int DT, int EPI, int BM, int BNW>
+__global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmParams p) {
+    using T = FTile<EPI, BM, BNW>;
+    typedef Elt<DT> E;
+    constexpr int NS = T::NS, NF = T::NF, WNT = T::WNT, NC = T::NC, ROWB = T::ROWB;
+    __shared__ __attribute__((aligned(16))) char lds[T::LDS_BYTES];
+
+    // ---- the tile of this block.  The eight XCDs (block id mod 8) each take one contiguous eighth of the real tile list,
+    //      cut on the device from the group sizes; surplus blocks of the worst-case grid exit. ----
+    int RT = 0;
+    if (p.group_offsets) {
+        for (int g = 0; g < p.G; ++g) RT += (p.group_offsets[g + 1] - p.group_offsets[g] + BM - 1) / BM;
+    } else {
+        RT = (p.max_rows + BM - 1) / BM;
+    }
+    const int CT = p.col_tiles;
+    const long long Tn = (long long)RT * CT;
+    int ct = 0, row_begin = 0, row_end = 0, expert = 0;
+    {
+        const int x = blockIdx.x & 7;
+        const long long q8 = Tn >> 3, r8 = Tn & 7;
+        const long long n = q8 + (x < r8 ? 1 : 0), start = x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8;
+        const long long i = blockIdx.x >> 3;
+        if (i >= n) {
+            // surplus block of the worst-case grid.  With zero_tail the grid has at least one more than the tiles on every
+            // XCD: those blocks clear the rows that belong to no group.
+            if (!T::QOUT && p.zero_tail && p.group_offsets) {
+                const long long per_xcd = (long long)(gridDim.x >> 3) - (q8 + (r8 ? 1 : 0));  // surplus blocks of an XCD, at least
+                const long long sid = (i - n) * 8 + x;
+                const int lo = p.group_offsets[0], hi = p.group_offsets[p.G];
+                if (i - n < per_xcd)
+                    for (long long r = sid; r < p.max_rows; r += per_xcd * 8)
+                        if (r < lo || r >= hi)
+                            for (int c = threadIdx.x; c < p.N_out; c += FTHREADS) ((bf16_t *)p.out)[r * p.ldo + c] = 0;
+            }
+            return;
+        }
+        const long long t = start + i;
+        // super-rows of rs row tiles: an XCD works on rs x (32 / rs) tiles at a time, which share their panels in its L2
+        const long long per = (long long)p.rs * CT;
+        const int sr = (int)(t / per);
+        const int rem = (int)(t - sr * per);
+        const int rin = min(p.rs, RT - sr * p.rs);
+        ct = rem / rin;
+        const int rt = sr * p.rs + (rem - ct * rin);
+        if (p.group_offsets) {
+            int tile0 = 0;
+            for (int g = 0; g < p.G; ++g) {
+                const int b = p.group_offsets[g], e = p.group_offsets[g + 1];
+                const int nt = (e - b + BM - 1) / BM;
+                if (rt < tile0 + nt) {
+                    row_begin = b + (rt - tile0) * BM;
+                    row_end = e;
+                    expert = g % p.n_experts;
+                    break;
+                }
+                tile0 += nt;
+            }
+        } else {
+            row_begin = rt * BM;
+            row_end = p.max_rows;
+        }
+    }
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave & 3, lwave = wave & 3;
+    const int nk = (p.K + QB - 1) / QB;
+    const int tail = p.K - (nk - 1) * QB;  // columns of the last slice (a multiple of 16)
+    auto xsw = [](int row) { return (row >> 1) & 7; };
+    auto src_row = [&](int prow) -> long long {
+        if (prow > row_end - 1) prow = row_end - 1;  // rows behind the group are computed from its last one, never stored
+        return p.gather ? (long long)(p.gather[prow] >> p.gather_shift) : (long long)prow;
+    };
+
+    // ---- operand fills: one instruction = 8 rows x 128 bytes ----
+    constexpr int NPX = BM / 8 / FLW, NPW = BNW / 8 / FLW, PP = NPX + NPW;
+    const u8 *a_src[NPX], *w_src[NPW];
+    const int lr = lane >> 3, lc = lane & 7;
+    auto setup_ptrs = [&]() {
+#pragma unroll
+        for (int j = 0; j < NPX; ++j) {
+            const int row = (lwave * NPX + j) * 8 + lr;
+            a_src[j] = p.a + src_row(row_begin + row) * p.lda + (lc ^ xsw(row)) * 16;
+        }
+        const u8 *wb = p.w + (long long)expert * p.w_expert_stride;
+#pragma unroll
+        for (int j = 0; j < NPW; ++j) {
+            const int row = (lwave * NPW + j) * 8 + lr;
+            int wrow;
+            if (T::GATED) {
+                // wave wq owns rows [wq * WNT, +WNT) of the slot: first the 'a' rows of its columns, then their 'b' rows
+                const int wq = row / WNT, within = row % WNT;
+                const int col = ct * NC + wq * (WNT / 2) + (within % (WNT / 2));
+                wrow = min(col, p.N_out - 1) + (within / (WNT / 2)) * p.b_row_offset;
+            } else {
+                wrow = min(ct * BNW + row, p.N_out - 1);
+            }
+            w_src[j] = wb + (long long)wrow * p.K + (lc ^ xsw(row)) * 16;
+        }
+    };
+    auto stage = [&](int buf, int kt) {
+        char *slot = lds + buf * T::SLOT;
+        if (kt == nk - 1 && tail < QB) {
+            const u8 *z = reinterpret_cast<const u8 *>(&g_fp8_zero);
+#pragma unroll
+            for (int j = 0; j < NPX; ++j) {
+                const int cs = lc ^ xsw((lwave * NPX + j) * 8 + lr);
+                glds16b(cs * 16 < tail ? a_src[j] + (long long)kt * QB : z, slot + (lwave * NPX + j) * 1024);
+            }
+#pragma unroll
+            for (int j = 0; j < NPW; ++j) {
+                const int cs = lc ^ xsw((lwave * NPW + j) * 8 + lr);
+                glds16b(cs * 16 < tail ? w_src[j] + (long long)kt * QB : z, slot + BM * QB + (lwave * NPW + j) * 1024);
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < NPX; ++j) glds16b(a_src[j] + (long long)kt * QB, slot + (lwave * NPX + j) * 1024);
+#pragma unroll
+        for (int j = 0; j < NPW; ++j) glds16b(w_src[j] + (long long)kt * QB, slot + BM * QB + (lwave * NPW + j) * 1024);
+    };
+    // ---- scales of the tile: waves 4-7.  Rows: dword (4 slices) kq of row r at XS + (kq * BM + r) * 4 ----
+    auto load_scales = [&]() {
+        const int t2 = tid - 256;
+        const int kq_n = (nk + 3) >> 2;
+        const int r = t2 & (BM - 1);
+        const u8 *src = p.a_scale + src_row(row_begin + r) * p.ld_as;
+        for (int kq = t2 / BM; kq < kq_n; kq += 256 / BM)
+            *reinterpret_cast<unsigned *>(lds + T::XS + (kq * BM + r) * 4) = *reinterpret_cast<const unsigned *>(src + kq * 4);
+        const u8 *wsb = p.w_scale + (long long)expert * p.ws_expert_stride;
+        const int nb = (p.N_out + QB - 1) / QB;
+        for (int i = t2; i < 2 * nk; i += 256) {
+            const int h = i >= nk ? 1 : 0, kb = i - h * nk;
+            int blk;
+            if (T::GATED) blk = min(ct * NC / QB, nb - 1) + h * p.b_blk_offset;
+            else blk = min(ct * BNW / QB + h, nb - 1);
+            lds[T::WS + h * FP8_WS_ROW + kb] = (char)wsb[(long long)blk * nk + kb];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+
+    const int fr = lane & 15, fq = lane >> 4;
+    const int koff0 = (fq ^ xsw(fr)) * 16, koff1 = ((4 + fq) ^ xsw(fr)) * 16;
+    const int w_off = BM * QB + (wn * WNT + fr) * QB;
+
+    auto tile_body = [&](auto mfw_c, auto loads_c, const int row_off) {
+        constexpr int MFW = decltype(mfw_c)::value;
+        constexpr bool LOADS = decltype(loads_c)::value != 0;
+        const int x_off = (row_off + fr) * QB;
+        f32x4_t acc[NF][MFW];
+#pragma unroll
+        for (int nf = 0; nf < NF; ++nf)
+#pragma unroll
+            for (int mf = 0; mf < MFW; ++mf) acc[nf][mf] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+        if (LOADS) {
+#pragma unroll
+            for (int s = 0; s < NS - 1; ++s)
+                if (s < nk) stage(s, s);
+        } else {
+            load_scales();
+        }
+        for (int kt = 0; kt < nk; ++kt) {
+            const int ahead = nk - 1 - kt;
+            static_assert((NS - 2) * PP < 64, "vmcnt field");
+            switch (ahead < NS - 2 ? ahead : NS - 2) {
+                case 0: fwait_vm_barrier<0>(); break;
+                case 1: fwait_vm_barrier<PP>(); break;
+                case 2: fwait_vm_barrier<(NS > 3 ? 2 : 0) * PP>(); break;
+                case 3: fwait_vm_barrier<(NS > 4 ? 3 : 0) * PP>(); break;
+                case 4: fwait_vm_barrier<(NS > 5 ? 4 : 0) * PP>(); break;
+                case 5: fwait_vm_barrier<(NS > 6 ? 5 : 0) * PP>(); break;
+                default: fwait_vm_barrier<(NS > 7 ? 6 : 0) * PP>(); break;
+            }
+            if (LOADS && kt + NS - 1 < nk) stage((kt + NS - 1) % NS, kt + NS - 1);
+            const char *lb = lds + (kt % NS) * T::SLOT;
+            const char *xs = lds + T::XS + ((kt >> 2) * BM + row_off + fr) * 4 + (kt & 3);
+            constexpr int PD = 2;  // X fragments read ahead
+            v8i_t wf[NF], xf[MFW];
+            int xsc[MFW], wsc[2];
+            auto ld32 = [&](const char *q) {
+                const v4i_t lo = *reinterpret_cast<const v4i_t *>(q + koff0), hi = *reinterpret_cast<const v4i_t *>(q + koff1);
+                return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+            auto ldx = [&](int t) {
+                xsc[t] = (int)*reinterpret_cast<const u8 *>(xs + t * 64);
+                xf[t] = ld32(lb + x_off + t * 16 * QB);
+            };
+            // plain: the wave's columns lie in one block of the weights' scales; gated: 'a' fragments in one, 'b' in the other
+            wsc[0] = (int)*reinterpret_cast<const u8 *>(lds + T::WS + (T::GATED ? 0 : (wn * WNT) / QB) * FP8_WS_ROW + kt);
+            wsc[1] = T::GATED ? (int)*reinterpret_cast<const u8 *>(lds + T::WS + FP8_WS_ROW + kt) : wsc[0];
+#pragma unroll
+            for (int nf = 0; nf < NF; ++nf) wf[nf] = ld32(lb + w_off + nf * 16 * QB);
+#pragma unroll
+            for (int t = 0; t < PD && t < MFW; ++t) ldx(t);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int t = 0; t < MFW; ++t) {
+                if (t + PD < MFW) ldx(t + PD);
+#pragma unroll
+                for (int nf = 0; nf < NF; ++nf)
+                    acc[nf][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        wf[nf], xf[t], acc[nf][t], 0, 0, 0, wsc[T::GATED && nf >= NF / 2 ? 1 : 0], 0, xsc[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+        }
+        __syncthreads();  // every wave is done reading the ring
+
+        const bf16_t *bias = p.bias ? p.bias + (long long)expert * p.bias_expert_stride : nullptr;
+        auto bias_at = [&](int c) { return c < p.N_out ? E::to_f(bias[c]) : 0.f; };
+        if constexpr (!T::QOUT) {
+#pragma unroll
+            for (int nf = 0; nf < NF; ++nf) {
+                const int cl = wn * WNT + nf * 16 + fq * 4, c0 = ct * NC + cl;
+                float bv[4] = {0.f, 0.f, 0.f, 0.f};
+                if (bias) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bv[j] = bias_at(c0 + j);
+                }
+#pragma unroll
+                for (int mf = 0; mf < MFW; ++mf) {
+                    uint2 o;
+                    o.x = E::pack2(acc[nf][mf][0] + bv[0], acc[nf][mf][1] + bv[1]);
+                    o.y = E::pack2(acc[nf][mf][2] + bv[2], acc[nf][mf][3] + bv[3]);
+                    *reinterpret_cast<uint2 *>(lds + (row_off + mf * 16 + fr) * ROWB + cl * 2) = o;
+                }
+            }
+        } else {
+            // activation in fp32, the maximum of every row's block of 128 columns over the four lanes of a row (shuffles) and
+            // over the waves of the block (LDS), then e4m3 into the image.  Columns behind N_out repeat the last real one:
+            // they belong to the same block, so its maximum is not changed, and they are not stored.
+            constexpr int HF = T::GATED ? NF / 2 : NF;         // output fragments of the wave
+            constexpr int CW = T::GATED ? WNT / 2 : WNT;       // output columns of the wave
+            constexpr int GW = QB / CW;                        // waves that share a block of 128 columns
+            unsigned *const top = reinterpret_cast<unsigned *>(lds + T::TOP);
+            unsigned mx[MFW];
+#pragma unroll
+            for (int mf = 0; mf < MFW; ++mf) mx[mf] = 0;
+#pragma unroll
+            for (int nf = 0; nf < HF; ++nf) {
+                const int c0 = ct * NC + wn * CW + nf * 16 + fq * 4;
+                float ba[4] = {0.f, 0.f, 0.f, 0.f}, bb[4] = {0.f, 0.f, 0.f, 0.f};
+                if (bias) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = min(c0 + j, p.N_out - 1);
+                        ba[j] = E::to_f(bias[c]);
+                        if (T::GATED) bb[j] = E::to_f(bias[p.b_row_offset + c]);
+                    }
+                }
+#pragma unroll
+                for (int mf = 0; mf < MFW; ++mf)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float a = acc[nf][mf][j] + ba[j];
+                        float h;
+                        if constexpr (T::GATED) {
+                            const float b = acc[nf + HF][mf][j] + bb[j];
+                            h = (c0 + j < p.n_gated ? fast_silu(a) : 1.0f) * b;
+                        } else {
+                            h = gelu_new_f32(a);
+                        }
+                        acc[nf][mf][j] = h;
+                        const unsigned u = abs_bits(h);
+                        mx[mf] = u > mx[mf] ? u : mx[mf];
+                    }
+            }
+#pragma unroll
+            for (int mf = 0; mf < MFW; ++mf) {
+                const unsigned m = umax_xor(umax_xor(mx[mf], 16), 32);
+                if (fq == 0) top[wn * BM + row_off + mf * 16 + fr] = m;
+            }
+            __syncthreads();
+            const int g0 = (wn / GW) * GW;
+#pragma unroll
+            for (int mf = 0; mf < MFW; ++mf) {
+                const int r = row_off + mf * 16 + fr;
+                unsigned m = 0;
+#pragma unroll
+                for (int w = 0; w < GW; ++w) {
+                    const unsigned o = top[(g0 + w) * BM + r];
+                    m = o > m ? o : m;
+                }
+                const unsigned sb = scale_byte(m);
+                const float inv = inv_scale(sb);
+                const int blk = (ct * NC + wn * CW) / QB;
+                if (wn == g0 && fq == 0 && row_begin + r < row_end && blk * QB < p.N_out)
+                    p.out_scale[(long long)(row_begin + r) * p.ld_os + blk] = (u8)sb;
+#pragma unroll
+                for (int nf = 0; nf < HF; ++nf)
+                    *reinterpret_cast<unsigned *>(lds + r * ROWB + wn * CW + nf * 16 + fq * 4) =
+                        pack_fp8x4(acc[nf][mf][0] * inv, acc[nf][mf][1] * inv, acc[nf][mf][2] * inv, acc[nf][mf][3] * inv);
+            }
+        }
+        __syncthreads();
+    };
+    constexpr int TF = BM / 16;
+    constexpr int AMF = TF / 2;
+    if (wave < FLW) {
+        setup_ptrs();
+        tile_body(FInt<AMF>{}, FInt<1>{}, 0);
+    } else {
+        tile_body(FInt<TF - AMF>{}, FInt<0>{}, AMF * 16);
+    }
+
+    // ---- image -> global, 16 bytes a lane ----
+    constexpr int EL = T::QOUT ? 16 : 8;  // elements per 16-byte chunk
+    constexpr int CPR = NC / EL, RPI = FTHREADS / CPR;
+    const int cc = tid % CPR, r0 = tid / CPR;
+    const int col = ct * NC + cc * EL;
+    const int left = p.N_out - col;
+    if (left <= 0) return;
+#pragma unroll 4
+    for (int r = r0; r < BM; r += RPI) {
+        const int prow = row_begin + r;
+        if (prow >= row_end) break;
+        typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+        const u32x4_t v = *reinterpret_cast<const u32x4_t *>(lds + r * ROWB + cc * 16);
+        if constexpr (T::QOUT) {
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t *>((u8 *)p.out + (long long)prow * p.ldo + col));
+        } else {
+            bf16_t *dst = (bf16_t *)p.out + (long long)prow * p.ldo + col;
+            if (left >= 8 && p.vec_store) {
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t *>(dst));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < left) dst[j] = (bf16_t)(v[j >> 1] >> ((j & 1) * 16));
+            }
+        }
+    }
+}
+
+template <int DT, int EPI, int BM, int BNW>
+static int launch_fp8_tile(Fp8GemmParams p, hipStream_t st) {
+    using T = FTile<EPI, BM, BNW>;
+    p.col_tiles = (p.N_out + T::NC - 1) / T::NC;
+    p.rs = p.col_tiles <= 8 ? 3 : 4;
+    const long long rt = p.group_offsets ? (long long)p.max_rows / BM + p.G : ((long long)p.max_rows + BM - 1) / BM;
+    const long long grid = (rt * p.col_tiles + 7) / 8 * 8 + (p.zero_tail ? 8 : 0);
+    if (grid > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "fp8 product: too many tiles (%lld)", grid);
+    hipLaunchKernelGGL((fp8_gemm_kernel<DT, EPI, BM, BNW>), dim3((unsigned)grid), dim3(FTHREADS), 0, st, p);
+    return check_launch("fp8_gemm_kernel");
+}
+
+template <int DT, int EPI>
+static int launch_fp8_gemm(const Fp8GemmParams &p, hipStream_t st) {
+    const int kq = ((p.K + QB - 1) / QB + 3) / 4 * 4;
+    const long long per = (p.max_rows + p.G - 1) / p.G;  // rows of an average group
+    const bool fits256 = 256 * kq <= FP8_STRIP, fits128 = 128 * kq <= FP8_STRIP, fits64 = 64 * kq <= FP8_STRIP;
+    if (per > 192 && fits256) return launch_fp8_tile<DT, EPI, 256, 256>(p, st);
+    if (per > 64 && fits128) return launch_fp8_tile<DT, EPI, 128, 256>(p, st);
+    if (per > 32 && fits64) return launch_fp8_tile<DT, EPI, 64, 256>(p, st);
+    return launch_fp8_tile<DT, EPI, 32, 256>(p, st);
+}
+
+static int fp8_gemm(const Fp8GemmParams &p, int epilogue, int dtype, hipStream_t st) {
+    if (p.max_rows == 0) return 0;
+#define FP8_EPI(DT_)                                                                   \
+    switch (epilogue) {                                                                \
+        case MOE_EPI_SWIGLU: return launch_fp8_gemm<DT_, EPI_SWIGLU>(p, st);           \
+        case MOE_EPI_GELU_NEW: return launch_fp8_gemm<DT_, EPI_GELU_NEW>(p, st);       \
+        default: return launch_fp8_gemm<DT_, EPI_PLAIN>(p, st);                        \
+    }
+    if (dtype == MOE_DTYPE_F16) { FP8_EPI(DT_F16) }
+    FP8_EPI(DT_BF16)
+#undef FP8_EPI
+}
+
+// shape, stride and alignment rules that every product shares; nothing is launched when one is broken
+static int fp8_args_ok(const char *fn, const void *a, int64_t lda, const void *a_scale, int64_t ld_as, int gather_shift,
+                       const void *w, const void *w_scale, const void *bias, int G, int n_experts, int max_rows, int K, int N) {
+    if (!a || !a_scale || !w || !w_scale) return fail(MOE_ERR_ARG, "%s: null pointer", fn);
+    if (K < 16 || (K & 15) || K > FP8_MAX_K) return fail(MOE_ERR_SHAPE, "%s: need K %% 16 == 0, 16 <= K <= %d (K=%d)", fn, FP8_MAX_K, K);
+    if (N < 1 || G < 1 || G > 4096 || n_experts < 1 || max_rows < 0 || gather_shift < 0 || gather_shift > 1)
+        return fail(MOE_ERR_SHAPE, "%s: need N >= 1, 1 <= G <= 4096, experts >= 1, rows >= 0 (N=%d G=%d experts=%d rows=%d)", fn, N, G, n_experts, max_rows);
+    if (lda < K || (lda & 15)) return fail(MOE_ERR_SHAPE, "%s: row stride %lld: need >= K and a multiple of 16", fn, (long long)lda);
+    const int kb = (K + QB - 1) / QB;
+    if (ld_as < kb || (ld_as & 3)) return fail(MOE_ERR_SHAPE, "%s: scale row stride %lld: need >= %d and a multiple of 4", fn, (long long)ld_as, kb);
+    if (!aligned16(a) || !aligned16(w)) return fail(MOE_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);
+    if (reinterpret_cast<uintptr_t>(a_scale) & 3) return fail(MOE_ERR_ALIGN, "%s: row scales must be 4-byte aligned", fn);
+    if (bias && (reinterpret_cast<uintptr_t>(bias) & 1)) return fail(MOE_ERR_ALIGN, "%s: bias must be 2-byte aligned", fn);
+    return 0;
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" int moe_grouped_gemm_fp8_fwd(const void *a, int64_t lda, const void *a_scale, int64_t ld_as, const int32_t *gather,
+                                        int gather_shift, const void *w, const void *w_scale, const void *bias,
+                                        const int32_t *group_offsets, int G, int n_experts_local, int max_rows, int K, int N,
+                                        int zero_tail, void *out, int64_t ldo, int dtype, void *stream) {
+    const char *fn = "moe_grouped_gemm_fp8_fwd";
+    if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
+    if (!out || (!group_offsets && G != 1)) return fail(MOE_ERR_ARG, "%s: null pointer", fn);
+    int rc = fp8_args_ok(fn, a, lda, a_scale, ld_as, gather_shift, w, w_scale, bias, G, n_experts_local, max_rows, K, N);
+    if (rc) return rc;
+    if (ldo < N) return fail(MOE_ERR_SHAPE, "%s: output row stride %lld < N", fn, (long long)ldo);
+    if (reinterpret_cast<uintptr_t>(out) & 1) return fail(MOE_ERR_ALIGN, "%s: out must be 2-byte aligned", fn);
+    const int nk = (K + QB - 1) / QB, nb = (N + QB - 1) / QB;
+    Fp8GemmParams p{};
+    p.a = (const u8 *)a; p.lda = lda; p.a_scale = (const u8 *)a_scale; p.ld_as = ld_as;
+    p.gather = gather; p.gather_shift = gather_shift;
+    p.w = (const u8 *)w; p.w_expert_stride = (long long)N * K;
+    p.w_scale = (const u8 *)w_scale; p.ws_expert_stride = (long long)nb * nk;
+    p.bias = (const bf16_t *)bias; p.bias_expert_stride = N;
+    p.group_offsets = group_offsets; p.G = G; p.n_experts = n_experts_local; p.max_rows = max_rows;
+    p.out = out; p.ldo = ldo; p.K = K; p.N_out = N; p.n_gated = N;
+    p.vec_store = aligned16(out) && (ldo & 7) == 0;
+    p.zero_tail = zero_tail != 0;
+    return fp8_gemm(p, MOE_EPI_PLAIN, dtype, (hipStream_t)stream);
+}
+
+namespace {
+inline size_t pad256b(size_t b) { return (b + 255) & ~(size_t)255; }
+struct FfnWs {
+    u8 *hq, *hs, *aq, *as;
+    long long ld_hs, ld_as;
+    size_t total;
+};
+FfnWs carve_ffn(void *ws, int src_rows, int max_rows, int M, int I) {
+    FfnWs r;
+    char *base = (char *)ws;
+    size_t off = 0;
+    auto take = [&](size_t bytes) { char *q = base + off; off += pad256b(bytes); return (u8 *)q; };
+    r.ld_hs = ((I + QB - 1) / QB + 3) / 4 * 4;
+    r.ld_as = ((M + QB - 1) / QB + 3) / 4 * 4;
+    r.hq = take((size_t)max_rows * I);
+    r.hs = take((size_t)max_rows * r.ld_hs);
+    r.aq = take((size_t)src_rows * M);
+    r.as = take((size_t)src_rows * r.ld_as);
+    r.total = off;
+    return r;
+}
+}  // namespace
+
+extern "C" size_t moe_expert_ffn_fp8_workspace_bytes(int src_rows, int max_rows, int M, int I) {
+    if (src_rows < 0 || max_rows < 0 || M < 1 || I < 1) return 0;
+    return carve_ffn(nullptr, src_rows, max_rows, M, I).total;
+}
+
+extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int src_rows, const void *a, int64_t lda,
+                                      const void *a_scale, int64_t ld_as, const int32_t *gather, int gather_shift,
+                                      const void *w1, const void *w1_scale, const void *b1, const void *w2,
+                                      const void *w2_scale, const void *b2, const int32_t *group_offsets, int G,
+                                      int n_experts_local, int max_rows, int M, int I, int n_gated, void *workspace,
+                                      size_t ws_bytes, void *y, int dtype, void *stream) {
+    const char *fn = "moe_expert_ffn_fp8_fwd";
+    if (act != MOE_ACT_SWIGLU && act != MOE_ACT_GELU_NEW) return fail(MOE_ERR_ARG, "%s: unknown act %d", fn, act);
+    if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
+    if ((!x) == (!a)) return fail(MOE_ERR_ARG, "%s: give either 16-bit rows x or 8-bit rows a", fn);
+    if (!group_offsets || !workspace || !y) return fail(MOE_ERR_ARG, "%s: null pointer", fn);
+    if (src_rows < 0 || max_rows < 0) return fail(MOE_ERR_SHAPE, "%s: negative row count", fn);
+    if (M < 16 || (M & 15) || I < 16 || (I & 15)) return fail(MOE_ERR_SHAPE, "%s: need M %% 16 == 0 and I %% 16 == 0 (M=%d I=%d)", fn, M, I);
+    if (!aligned16(workspace) || !aligned16(y)) return fail(MOE_ERR_ALIGN, "%s: workspace and y must be 16-byte aligned", fn);
+    const FfnWs ws = carve_ffn(workspace, x ? src_rows : 0, max_rows, M, I);
+    if (ws_bytes < ws.total) return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, ws_bytes, ws.total);
+    if (x) { a = max_rows ? ws.aq : workspace; lda = M; a_scale = max_rows ? ws.as : workspace; ld_as = ws.ld_as; }
+    int rc = fp8_args_ok(fn, a, lda, a_scale, ld_as, gather_shift, w1, w1_scale, b1, G, n_experts_local, max_rows, M, I);
+    if (rc) return rc;
+    rc = fp8_args_ok(fn, workspace, I, workspace, ws.ld_hs, 0, w2, w2_scale, b2, G, n_experts_local, max_rows, I, M);
+    if (rc) return rc;
+    if (max_rows == 0) return 0;
+    if (x && (rc = moe_quantize_rows_fp8(x, ldx, src_rows, M, ws.aq, M, ws.as, ws.ld_as, dtype, stream))) return rc;
+    const bool gated = act == MOE_ACT_SWIGLU;
+    const int mb = (M + QB - 1) / QB, ib = (I + QB - 1) / QB;
+    Fp8GemmParams p{};
+    p.a = (const u8 *)a; p.lda = lda; p.a_scale = (const u8 *)a_scale; p.ld_as = ld_as;
+    p.gather = gather; p.gather_shift = gather_shift;
+    p.w = (const u8 *)w1; p.w_expert_stride = (long long)(gated ? 2 : 1) * I * M;
+    p.w_scale = (const u8 *)w1_scale; p.ws_expert_stride = (long long)(gated ? 2 : 1) * ib * mb;
+    p.bias = (const bf16_t *)b1; p.bias_expert_stride = (gated ? 2 : 1) * (long long)I;
+    p.group_offsets = group_offsets; p.G = G; p.n_experts = n_experts_local; p.max_rows = max_rows;
+    p.out = ws.hq; p.ldo = I; p.out_scale = ws.hs; p.ld_os = ws.ld_hs;
+    p.K = M; p.N_out = I; p.b_row_offset = I; p.b_blk_offset = ib;
+    p.n_gated = (n_gated < 0 || n_gated > I) ? I : n_gated;
+    if ((rc = fp8_gemm(p, gated ? MOE_EPI_SWIGLU : MOE_EPI_GELU_NEW, dtype, (hipStream_t)stream))) return rc;
+    return moe_grouped_gemm_fp8_fwd(ws.hq, I, ws.hs, ws.ld_hs, nullptr, 0, w2, w2_scale, b2, group_offsets, G, n_experts_local,
+                                    max_rows, I, M, 0, y, M, dtype, stream);
+}

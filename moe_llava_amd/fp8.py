@@ -1,0 +1,351 @@
+"""8-bit experts: products and expert MLPs on e4m3 operands with power-of-two scales per block of 128.
+
+Format (``include/moe_gfx950.h``): e4m3 elements (``torch.float8_e4m3fn``) and, for every 1 x 128 block of a row and every
+128 x 128 block of a weight matrix, one scale 2^e held as ``torch.float8_e8m0fnu``; e is the smallest exponent that brings
+the block's largest magnitude to 448 or below, so that scaling rounds nothing.
+
+    w, ws = fp8.quantize_weight(weight)              # [.., N, K] bf16 / fp16 -> e4m3 + scales, once
+    y = fp8.linear(x, w, ws, bias)                   # x [.., K]; differentiable with respect to x (weights are frozen)
+    y = fp8.grouped_linear(x, w, ws, group_offsets)  # rows of group g with expert g % E
+    y = fp8.expert_ffn("swiglu", x, w1, ws1, w2, ws2, group_offsets, max_rows, gather, 1)      # inference
+
+Inputs are 16-bit tensors, quantised in front of the product, or ``Fp8Rows`` (``quantize_rows``, ``norm.add_rms_norm_fp8``).
+The reference has no counterpart: its experts run in 16 bits.  As in ``ops``, nothing here computes on the CPU.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib, ops
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+E8M0 = torch.float8_e8m0fnu
+MAX_K = 65536            # columns of a product's operands
+_ACTS = {"swiglu": ops.ACT_SWIGLU, "gelu_new": ops.ACT_GELU_NEW, ops.ACT_SWIGLU: ops.ACT_SWIGLU,
+         ops.ACT_GELU_NEW: ops.ACT_GELU_NEW}
+
+
+class Fp8Rows(NamedTuple):
+    """Rows in 8 bits: ``q`` [S, K] e4m3 and ``scale`` [S, ceil(K/128)] e8m0.  The scales' row stride is a multiple of 4
+    bytes (``scale`` is a view of a padded buffer), as the kernels read them 4 at a time."""
+    q: Tensor
+    scale: Tensor
+
+
+def _blocks(n: int) -> int:
+    return (n + BLOCK - 1) // BLOCK
+
+
+def _empty_rows(S: int, K: int, dev) -> Fp8Rows:
+    kb = _blocks(K)
+    q = torch.empty((S, K), dtype=E4M3, device=dev)
+    sc = torch.empty((S, (kb + 3) // 4 * 4), dtype=E8M0, device=dev)
+    return Fp8Rows(q, sc[:, :kb] if kb % 4 else sc)
+
+
+def _gpu(t, name: str) -> None:
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if not t.is_cuda:
+        raise _lib.MoEKernelError(f"{name}: must live on the GPU (got {t.device}); there is no CPU path")
+
+
+def _half_rows(x: Tensor, name: str) -> Tensor:
+    """x [.., K] as rows [S, K] whose last dimension is dense (other strides stay; a copy only where they cannot)."""
+    _gpu(x, name)
+    if x.dtype not in ops.HALF_DTYPES:
+        raise TypeError(f"{name}: expected bf16 or fp16, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError(f"{name}: expected at least one dimension")
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(x.shape[:-1].numel(), x.shape[-1])
+    if x.shape[1] > 1 and x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()                  # transposed, or rows that overlap (an expanded row)
+    return x
+
+
+def _check_rows(a: Fp8Rows, name: str) -> Fp8Rows:
+    q, sc = a
+    _gpu(q, f"{name}.q")
+    _gpu(sc, f"{name}.scale")
+    if q.dtype != E4M3 or sc.dtype != E8M0 or q.dim() != 2 or sc.dim() != 2:
+        raise TypeError(f"{name}: expected e4m3 rows [S, K] and e8m0 scales [S, ceil(K/128)]")
+    S, K = q.shape
+    if tuple(sc.shape) != (S, _blocks(K)) or sc.device != q.device:
+        raise ValueError(f"{name}: scales {tuple(sc.shape)} on {sc.device} do not match rows {tuple(q.shape)} on {q.device}")
+    if q.stride(1) != 1 or (S > 1 and (q.stride(0) % 16 or q.stride(0) < K)) or q.data_ptr() % 16:
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+    kb4 = (sc.shape[1] + 3) // 4 * 4
+    room = sc.untyped_storage().nbytes() - sc.storage_offset()      # e8m0: one byte per element
+    st = sc.stride(0) if S > 1 else kb4
+    if sc.stride(1) != 1 and sc.shape[1] > 1 or st % 4 or st < kb4 or sc.data_ptr() % 4 or room < (S - 1) * st + kb4:
+        pad = torch.empty((S, kb4), dtype=E8M0, device=q.device)
+        pad.view(torch.uint8)[:, :sc.shape[1]].copy_(sc.view(torch.uint8))
+        sc = pad[:, :sc.shape[1]]
+    return Fp8Rows(q, sc)
+
+
+def _lead(t: Tensor, width: int) -> int:
+    """Row stride of a 2-d tensor; that of a single row is arbitrary in torch."""
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def _lead_scale(sc: Tensor) -> int:
+    return sc.stride(0) if sc.shape[0] > 1 else (sc.shape[1] + 3) // 4 * 4
+
+
+def _check_weight(w: Tensor, ws: Tensor, name: str, E: int, N: Optional[int], parts: int = 1) -> Tuple[int, int]:
+    """w [E, parts*N, K] with scales [E, parts*ceil(N/128), ceil(K/128)]; returns (N, K)."""
+    for t, n, dt in ((w, name, E4M3), (ws, f"{name}_scale", E8M0)):
+        _gpu(t, n)
+        if t.dtype != dt:
+            raise TypeError(f"{n}: expected {dt}, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{n}: must be contiguous")
+    n, K = w.shape[-2], w.shape[-1]
+    if n % parts or (N is not None and n != parts * N):
+        raise ValueError(f"{name}: {tuple(w.shape)} does not hold {parts} projection(s) of the expected width")
+    n //= parts
+    if K % 16 or not 16 <= K <= MAX_K:
+        raise ValueError(f"{name}: K={K} must be a multiple of 16 and at most {MAX_K}")
+    if ws.device != w.device or tuple(ws.shape) != tuple(w.shape[:-2]) + (parts * _blocks(n), _blocks(K)):
+        raise ValueError(f"{name}_scale: {tuple(ws.shape)} on {ws.device} does not match {name} {tuple(w.shape)} on {w.device}")
+    if w.dim() == 3 and w.shape[0] != E:
+        raise ValueError(f"{name}: {w.shape[0]} experts, expected {E}")
+    if w.data_ptr() % 16:
+        raise ValueError(f"{name}: must be 16-byte aligned")
+    return n, K
+
+
+def _check_bias(b: Optional[Tensor], name: str, shape, dtype, dev) -> None:
+    if b is None:
+        return
+    if not isinstance(b, Tensor) or b.dtype != dtype or tuple(b.shape) != tuple(shape) or b.device != dev \
+            or not b.is_contiguous():
+        raise ValueError(f"{name}: need a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
+
+
+def _check_index(t: Tensor, name: str, dev) -> None:
+    _gpu(t, name)
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name}: need a contiguous 1-d int32 tensor on {dev}")
+
+
+# ------------------------------------------------------------------------------------------------ quantisation
+def quantize_rows(x: Tensor) -> Fp8Rows:
+    """16-bit rows [.., K] (any row stride, K % 16 == 0) -> ``Fp8Rows`` of shape [S, K]."""
+    x = _half_rows(x, "x")
+    S, K = x.shape
+    if K % 16 or K < 16:
+        raise ValueError(f"x: K={K} must be a multiple of 16")
+    out = _empty_rows(S, K, x.device)
+    if S:
+        with ops._on(x.device):
+            rc = _lib.load().moe_quantize_rows_fp8(x.data_ptr(), _lead(x, K), S, K, out.q.data_ptr(), K, out.scale.data_ptr(),
+                                                   _lead_scale(out.scale), ops._dt(x), ops._stream_ptr(x))
+        _lib.check(rc, "moe_quantize_rows_fp8")
+    return out
+
+
+def quantize_weight(w: Tensor, projections: int = 1) -> Tuple[Tensor, Tensor]:
+    """16-bit weights [.., N, K] (K % 16 == 0) -> (e4m3 [.., N, K], scales [.., projections * ceil(N'/128), ceil(K/128)]).
+    ``projections`` = 2 for a gated W1 [.., 2I, M]: each half gets blocks of its own (N' = I)."""
+    _gpu(w, "w")
+    if w.dtype not in ops.HALF_DTYPES:
+        raise TypeError(f"w: expected bf16 or fp16, got {w.dtype}")
+    if w.dim() < 2 or w.numel() == 0 or w.shape[-2] % projections or w.shape[-1] % 16:
+        raise ValueError(f"w: {tuple(w.shape)}: need [.., N, K] with K % 16 == 0 and N a multiple of {projections}")
+    w = w.contiguous()
+    if w.data_ptr() % 16:
+        w = w.clone()
+    n, k = w.shape[-2] // projections, w.shape[-1]
+    batch = w.numel() // (n * k)
+    q = torch.empty(w.shape, dtype=E4M3, device=w.device)
+    sc = torch.empty(tuple(w.shape[:-2]) + (projections * _blocks(n), _blocks(k)), dtype=E8M0, device=w.device)
+    with ops._on(w.device):
+        rc = _lib.load().moe_quantize_blocks_fp8(w.data_ptr(), batch, n, k, q.data_ptr(), sc.data_ptr(), ops._dt(w),
+                                                 ops._stream_ptr(w))
+    _lib.check(rc, "moe_quantize_blocks_fp8")
+    return q, sc
+
+
+# ------------------------------------------------------------------------------------------------ products
+def _gemm(a: Fp8Rows, w: Tensor, ws: Tensor, bias: Optional[Tensor], offs: Optional[Tensor], E: int, N: int, K: int, dtype,
+          zero_tail: bool) -> Tensor:
+    S = a.q.shape[0]
+    out = torch.empty((S, N), dtype=dtype, device=a.q.device)
+    if S == 0:
+        return out
+    G = offs.numel() - 1 if offs is not None else 1
+    with ops._on(a.q.device):
+        rc = _lib.load().moe_grouped_gemm_fp8_fwd(
+            a.q.data_ptr(), _lead(a.q, K), a.scale.data_ptr(), _lead_scale(a.scale), None, 0, w.data_ptr(), ws.data_ptr(),
+            bias.data_ptr() if bias is not None else None, offs.data_ptr() if offs is not None else None, G, E, S, K, N,
+            int(zero_tail), out.data_ptr(), N, ops.DTYPE_F16 if dtype == torch.float16 else ops.DTYPE_BF16,
+            ops._stream_ptr(a.q))
+    _lib.check(rc, "moe_grouped_gemm_fp8_fwd")
+    return out
+
+
+class _LinearFn(torch.autograd.Function):
+    """y = Q(x) W^T + b over groups of rows; dx = Q(dy) W with W's blocks transposed on the fly (frozen weights: no copy of
+    them is kept).  The rounding of x to 8 bits is passed through as the identity; a gradient of ``bias`` is the column sum
+    of dy and is refused here (8-bit experts are frozen)."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, w: Tensor, ws: Tensor, bias, offs, E: int, N: int, K: int):
+        ctx.save_for_backward(w, ws, offs)
+        ctx.meta = (E, N, K, x.shape, x.dtype)
+        return _gemm(quantize_rows(x), w, ws, bias, offs, E, N, K, x.dtype, offs is not None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy: Tensor):
+        w, ws, offs = ctx.saved_tensors
+        E, N, K, shape, dtype = ctx.meta
+        wt = torch.empty((E, K, N), dtype=E4M3, device=w.device)
+        wst = torch.empty((E, _blocks(K), _blocks(N)), dtype=E8M0, device=w.device)
+        with ops._on(w.device):
+            rc = _lib.load().moe_transpose_blocks_fp8(w.data_ptr(), ws.data_ptr(), E, N, K, wt.data_ptr(), wst.data_ptr(),
+                                                      ops._stream_ptr(w))
+        _lib.check(rc, "moe_transpose_blocks_fp8")
+        dx = _gemm(quantize_rows(dy), wt, wst, None, offs, E, K, N, dtype, offs is not None)
+        return dx.reshape(shape), None, None, None, None, None, None, None
+
+
+def _linear(x, w: Tensor, ws: Tensor, bias: Optional[Tensor], offs: Optional[Tensor], dtype) -> Tensor:
+    E = w.shape[0] if offs is not None else 1
+    if w.dim() != (3 if offs is not None else 2):
+        raise ValueError(f"w: {tuple(w.shape)}: need {'[E, N, K]' if offs is not None else '[N, K]'}")
+    N, K = _check_weight(w, ws, "w", E, None)
+    if isinstance(x, Fp8Rows):
+        if dtype is None:
+            dtype = bias.dtype if bias is not None else torch.bfloat16
+        if dtype not in ops.HALF_DTYPES:
+            raise TypeError(f"out_dtype: expected bf16 or fp16, got {dtype}")
+        rows = _check_rows(x, "x")
+        if rows.q.shape[1] != K or rows.q.device != w.device:
+            raise ValueError(f"x {tuple(rows.q.shape)} on {rows.q.device} does not match w {tuple(w.shape)} on {w.device}")
+    else:
+        if dtype is not None and dtype != x.dtype:
+            raise TypeError("out_dtype is the input's type for 16-bit inputs")
+        rows = None
+        dtype = x.dtype
+        x2 = _half_rows(x, "x")
+        if x2.shape[1] != K or x2.device != w.device:
+            raise ValueError(f"x {tuple(x.shape)} on {x2.device} does not match w {tuple(w.shape)} on {w.device}")
+    _check_bias(bias, "bias", (E, N) if offs is not None else (N,), dtype, w.device)
+    if offs is not None:
+        _check_index(offs, "group_offsets", w.device)
+        if not 1 <= offs.numel() - 1 <= 4096:
+            raise ValueError("group_offsets needs 2 to 4097 entries")
+    if rows is not None:
+        return _gemm(rows, w, ws, bias, offs, E, N, K, dtype, offs is not None)
+    if torch.is_grad_enabled():
+        if bias is not None and bias.requires_grad:
+            raise NotImplementedError("fp8 products are for frozen weights: bias.requires_grad is not supported")
+        if x.requires_grad:
+            if N % 16 or N > MAX_K:
+                raise NotImplementedError(f"the input gradient needs N % 16 == 0 and N <= {MAX_K} (N={N})")
+            y = _LinearFn.apply(x2, w, ws, bias, offs, E, N, K)
+            return y.reshape(x.shape[:-1] + (N,))
+    y = _gemm(quantize_rows(x2), w, ws, bias, offs, E, N, K, dtype, offs is not None)
+    return y.reshape(x.shape[:-1] + (N,))
+
+
+def linear(x: Union[Tensor, Fp8Rows], w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = None, out_dtype=None) -> Tensor:
+    """``x @ w.T + bias`` with w [N, K] in 8 bits.  x [.., K] bf16 / fp16 (the output's type), or ``Fp8Rows`` (``out_dtype``,
+    by default the bias' type, else bf16).  fp32 accumulation, one rounding.  Differentiable with respect to a 16-bit x when
+    N % 16 == 0: the gradient is quantised like any rows and multiplied by the transposed 8-bit weights."""
+    return _linear(x, w, w_scale, bias, None, out_dtype)
+
+
+def grouped_linear(x: Union[Tensor, Fp8Rows], w: Tensor, w_scale: Tensor, group_offsets: Tensor,
+                   bias: Optional[Tensor] = None, out_dtype=None) -> Tensor:
+    """``linear`` for ragged groups of rows: rows [group_offsets[g], group_offsets[g+1]) of x [S, K] use expert g % E of
+    w [E, N, K] (bias [E, N]).  ``group_offsets`` [G+1] int32 stays on the device (ascending, within [0, S]); rows of no
+    group give 0, and get no gradient."""
+    if not isinstance(x, Fp8Rows) and isinstance(x, Tensor) and x.dim() != 2:
+        raise ValueError(f"x: expected [S, K], got {tuple(x.shape)}")
+    if group_offsets is None:
+        raise ValueError("group_offsets is missing")
+    return _linear(x, w, w_scale, bias, group_offsets, out_dtype)
+
+
+# ------------------------------------------------------------------------------------------------ expert MLP
+def expert_ffn(act, x: Union[Tensor, Fp8Rows], w1: Tensor, w1_scale: Tensor, w2: Tensor, w2_scale: Tensor,
+               group_offsets: Tensor, max_rows: int, gather: Optional[Tensor] = None, gather_shift: int = 0,
+               b1: Optional[Tensor] = None, b2: Optional[Tensor] = None, n_gated: int = -1, out_dtype=None) -> Tensor:
+    """``ops.expert_ffn`` on 8-bit experts (inference): y [max_rows, M] for the compact rows of the groups; compact row p
+    reads row ``gather[p] >> gather_shift`` of x (row p without ``gather``); rows past ``group_offsets[G]`` are left
+    unwritten.  ``act`` "swiglu" (w1 [E, 2I, M], scales [E, 2*ceil(I/128), ceil(M/128)]) or "gelu_new" (w1 [E, I, M]);
+    w2 [E, M, I].  M and I are multiples of 16.  The activation is evaluated in fp32 on the first product's accumulators and
+    quantised per 128 hidden channels."""
+    act = _ACTS.get(act, -1)
+    if act < 0:
+        raise ValueError("act: 'swiglu' or 'gelu_new'")
+    if w1.dim() != 3 or w2.dim() != 3:
+        raise ValueError("w1 / w2: expected [E, N, K]")
+    E = w2.shape[0]
+    M, I = _check_weight(w2, w2_scale, "w2", E, None)
+    parts = 2 if act == ops.ACT_SWIGLU else 1
+    if _check_weight(w1, w1_scale, "w1", E, I, parts)[1] != M or M % 16 or I % 16:
+        raise ValueError(f"w1 {tuple(w1.shape)} / w2 {tuple(w2.shape)} do not match (multiples of 16)")
+    dev = w1.device
+    eight = isinstance(x, Fp8Rows)
+    if eight:
+        x = _check_rows(x, "x")
+        src = x.q
+        dtype = out_dtype or (b2.dtype if b2 is not None else torch.bfloat16)
+        if dtype not in ops.HALF_DTYPES:
+            raise TypeError(f"out_dtype: expected bf16 or fp16, got {dtype}")
+    else:
+        x = src = _half_rows(x, "x")
+        dtype = x.dtype
+        if out_dtype is not None and out_dtype != dtype:
+            raise TypeError("out_dtype is the input's type for 16-bit inputs")
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise NotImplementedError("fp8.expert_ffn is for inference: wrap it in torch.no_grad(), or compose "
+                                      "fp8.grouped_linear, which is differentiable")
+    if src.shape[1] != M or src.device != dev or w2.device != dev:
+        raise ValueError(f"x {tuple(src.shape)} on {src.device} does not match w1 {tuple(w1.shape)} on {dev}")
+    _check_bias(b1, "b1", (E, parts * I), dtype, dev)
+    _check_bias(b2, "b2", (E, M), dtype, dev)
+    _check_index(group_offsets, "group_offsets", dev)
+    G = group_offsets.numel() - 1
+    if not 1 <= G <= 4096 or max_rows < 0:
+        raise ValueError("group_offsets needs 2 to 4097 entries, max_rows >= 0")
+    if gather is not None:
+        _check_index(gather, "gather", dev)
+        if gather.numel() < max_rows:
+            raise ValueError("gather shorter than max_rows")
+        if gather_shift not in (0, 1):
+            raise ValueError("gather_shift: 0 or 1")
+    elif src.shape[0] < max_rows:
+        raise ValueError("x has fewer rows than max_rows")
+    y = torch.empty((max_rows, M), dtype=dtype, device=dev)
+    if max_rows == 0:
+        return y
+    S = src.shape[0]
+    lib = _lib.load()
+    nws = lib.moe_expert_ffn_fp8_workspace_bytes(0 if eight else S, max_rows, M, I)
+    ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
+    if eight:
+        args = (None, 0, 0, src.data_ptr(), _lead(src, M), x.scale.data_ptr(), _lead_scale(x.scale))
+    else:
+        args = (src.data_ptr(), _lead(src, M), S, None, 0, None, 0)
+    with ops._on(dev):
+        rc = lib.moe_expert_ffn_fp8_fwd(
+            act, *args, gather.data_ptr() if gather is not None else None, gather_shift, w1.data_ptr(), w1_scale.data_ptr(),
+            b1.data_ptr() if b1 is not None else None, w2.data_ptr(), w2_scale.data_ptr(),
+            b2.data_ptr() if b2 is not None else None, group_offsets.data_ptr(), G, E, max_rows, M, I, n_gated,
+            ws.data_ptr(), nws, y.data_ptr(), ops.DTYPE_F16 if dtype == torch.float16 else ops.DTYPE_BF16,
+            ops._stream_ptr(src))
+    _lib.check(rc, "moe_expert_ffn_fp8_fwd")
+    return y

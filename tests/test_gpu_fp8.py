@@ -1,0 +1,404 @@
+"""Products and expert MLPs on e4m3 operands (moe_llava_amd.fp8) against 64 bits; the bounds are derived in _fp8_ref."""
+import pytest
+import torch
+
+from moe_llava_amd import _lib, fp8, norm, ops
+from tests import _fp8_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+D = torch.float64
+
+
+def _rows(g, S, K, dt, scale=1.0):
+    x = torch.randn((S, K), generator=g) * scale
+    if K > 40:
+        x[:, K // 3] *= 15
+    return x.to(dt)
+
+
+# ------------------------------------------------------------------------------------------------ quantisation
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("S,K", [(1, 16), (1, 2048), (3, 144), (130, 1008), (1000, 256), (2, 10240)])
+def test_quantize_rows_is_exact(S, K, dt):
+    g = torch.Generator().manual_seed(S + K)
+    x = _rows(g, S, K, dt)
+    x[0, 0] = 0.875 if K == 16 else x[0, 0]          # 448 = 0.875 * 2^9: the edge between two exponents
+    if S > 2:
+        x[1] = 0
+        x[2] = torch.sign(x[2]) * 1.75
+    q, b = R.quant(x)
+    for view in (x.to(DEV), torch.nn.functional.pad(x, (3, 5)).to(DEV)[:, 3:3 + K]):        # the second rules wide loads out
+        rows = fp8.quantize_rows(view)
+        assert torch.equal(rows.scale.cpu().view(torch.uint8).to(torch.int64), b)
+        assert torch.equal(rows.q.cpu().to(torch.float32).to(D), q)
+
+
+def test_quantize_rows_extremes():
+    x = torch.zeros((5, 256), dtype=torch.bfloat16)
+    x[0, 3] = float("inf")
+    x[1, 200] = float("nan")
+    x[2] = 3.3e38
+    x[3] = 1e-38
+    x[4, 0], x[4, 1] = 448.0, 2.0 ** -9              # the largest and the smallest e4m3 magnitudes side by side
+    r = fp8.quantize_rows(x.to(DEV))
+    q, b = r.q.cpu().to(torch.float32), r.scale.cpu().view(torch.uint8)
+    assert bool(torch.isnan(q[0, :128]).all()) and int(b[0, 0]) == 255 and not bool(q[0, 128:].any())
+    assert not bool(q[1, :128].any()) and bool(torch.isnan(q[1, 128:]).all()) and int(b[1, 1]) == 255
+    qr, br = R.quant(x[2:])
+    assert torch.equal(b[2:].to(torch.int64), br) and torch.equal(q[2:].to(D), qr)
+
+
+@pytest.mark.parametrize("parts,E,n,k", [(1, 1, 1, 16), (1, 3, 200, 144), (2, 2, 176, 256), (1, 2, 128, 1040)])
+def test_quantize_weight_is_exact(parts, E, n, k):
+    g = torch.Generator().manual_seed(n)
+    w = (torch.randn((E, parts * n, k), generator=g) * 0.1).to(torch.bfloat16)
+    q, s = fp8.quantize_weight(w.to(DEV), parts)
+    assert tuple(s.shape) == (E, parts * R.nb(n), R.nb(k))
+    for e in range(E):
+        for p in range(parts):
+            rq, rb = R.quant(w[e, p * n:(p + 1) * n], 128)
+            assert torch.equal(q[e, p * n:(p + 1) * n].cpu().to(torch.float32).to(D), rq)
+            assert torch.equal(s[e, p * R.nb(n):(p + 1) * R.nb(n)].cpu().view(torch.uint8).to(torch.int64), rb)
+
+
+# ------------------------------------------------------------------------------------------------ products
+SHAPES = [(1, 16, 1), (1, 2048, 64), (3, 144, 7), (16, 128, 300), (17, 1008, 1003), (33, 272, 129), (64, 256, 256),
+          (65, 528, 515), (100, 2064, 260), (129, 400, 640), (300, 640, 384), (513, 1280, 512), (700, 96, 1000),
+          (40, 16384, 48), (260, 14976, 64)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("S,K,N", SHAPES)
+def test_linear(S, K, N, dt):
+    g = torch.Generator().manual_seed(S * 3 + K + N)
+    x = _rows(g, S, K, dt)
+    q, s = R.weights(g, 1, N, K)
+    bias = torch.randn(N, generator=g).to(dt) if N % 2 else None
+    y = fp8.linear(x.to(DEV), q[0].to(DEV), s[0].to(DEV), bias.to(DEV) if bias is not None else None)
+    ref, tol = R.product(R.deq(x), R.deq_stored(q[0], s[0]))
+    if bias is not None:
+        ref = ref + bias.to(D)
+    R.check16(y, ref, tol, "linear")
+    # 8-bit rows give the same bits as the 16-bit rows they came from
+    y2 = fp8.linear(fp8.quantize_rows(x.to(DEV)), q[0].to(DEV), s[0].to(DEV), bias.to(DEV) if bias is not None else None, out_dtype=dt)
+    assert torch.equal(y, y2)
+
+
+@pytest.mark.parametrize("S,K,N", [(1, 64, 16), (37, 208, 144), (300, 512, 272), (70, 1040, 640)])
+def test_linear_input_gradient(S, K, N):
+    g = torch.Generator().manual_seed(S + K + N)
+    x, dy = _rows(g, S, K, torch.bfloat16), _rows(g, S, N, torch.bfloat16, 0.1)
+    q, s = R.weights(g, 1, N, K)
+    xg = x.to(DEV).view(1, S, K).requires_grad_(True)
+    y = fp8.linear(xg, q[0].to(DEV), s[0].to(DEV))
+    dx, = torch.autograd.grad(y, xg, dy.to(DEV).view(1, S, N))
+    w = R.deq_stored(q[0], s[0])
+    ref, tol = R.product(R.deq(dy), w.t().contiguous())
+    R.check16(dx.view(S, K), ref, tol, "dx")
+    # against differences of the unquantised function: what is between them is dy's rounding to 8 bits, half a step of e4m3
+    # (2^-4 of the value, or 2^-10 of the block's scale near zero)
+    d = torch.randn((S, K), generator=g, dtype=D)
+    xs = x.to(D)
+
+    def loss(v):
+        return ((v @ w.t()) * dy.to(D)).sum()
+    h = 1.0
+    diff = (loss(xs + h * d) - loss(xs - h * d)) / (2 * h)
+    unit = R.spread(torch.exp2(R.quant(dy)[1].to(D) - 127), S, N)
+    edy = torch.maximum(dy.to(D).abs() * 2.0 ** -4, unit * 2.0 ** -10)
+    lim = ((edy @ w.abs() + tol + R.half_step(torch.bfloat16) * (ref.abs() + tol)) * d.abs()).sum()
+    assert abs(float((dx.view(S, K).cpu().to(D) * d).sum() - diff)) <= float(lim) + 1e-9 * abs(float(diff))
+
+
+def _groups(g, S, G, lead=0, tail=0):
+    cut = torch.sort(torch.randint(lead, S - tail + 1, (G - 1,), generator=g)).values.tolist() if G > 1 else []
+    return torch.tensor([lead] + cut + [S - tail], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("E,G,S,K,N,lead,tail", [(3, 3, 50, 144, 72, 0, 0), (4, 8, 700, 256, 272, 5, 11), (2, 2, 1, 64, 16, 0, 0),
+                                               (8, 8, 900, 384, 400, 0, 300), (2, 6, 40, 528, 33, 39, 0), (5, 5, 300, 128, 520, 0, 0)])
+def test_grouped_linear(E, G, S, K, N, lead, tail):
+    g = torch.Generator().manual_seed(E * 100 + S)
+    x = _rows(g, S, K, torch.bfloat16)
+    q, s = R.weights(g, E, N, K)
+    bias = torch.randn((E, N), generator=g).to(torch.bfloat16)
+    offs = _groups(g, S, G, lead, tail)
+    if G == 5:
+        offs[2] = offs[1]                       # an empty group
+    ref, tol = torch.zeros((S, N), dtype=D), torch.zeros((S, N), dtype=D)
+    for i in range(G):
+        a, b = int(offs[i]), int(offs[i + 1])
+        if b > a:
+            r, t = R.product(R.deq(x[a:b]), R.deq_stored(q[i % E], s[i % E]))
+            ref[a:b], tol[a:b] = r + bias[i % E].to(D), t
+    y = fp8.grouped_linear(x.to(DEV), q.to(DEV), s.to(DEV), offs.to(DEV), bias.to(DEV))
+    R.check16(y, ref, tol, "grouped")           # rows of no group are exactly 0
+    assert not bool(y[:lead].any()) and not bool(y[S - tail:].any() if tail else False)
+    if N % 16 == 0:
+        xg = x.to(DEV).requires_grad_(True)
+        dy = _rows(g, S, N, torch.bfloat16)
+        dx, = torch.autograd.grad(fp8.grouped_linear(xg, q.to(DEV), s.to(DEV), offs.to(DEV), bias.to(DEV)), xg, dy.to(DEV))
+        rd, td = torch.zeros((S, K), dtype=D), torch.zeros((S, K), dtype=D)
+        for i in range(G):
+            a, b = int(offs[i]), int(offs[i + 1])
+            if b > a:
+                rd[a:b], td[a:b] = R.product(R.deq(dy[a:b]), R.deq_stored(q[i % E], s[i % E]).t().contiguous())
+        R.check16(dx, rd, td, "grouped dx")
+
+
+def test_strides_of_rows_scales_and_biases():
+    g = torch.Generator().manual_seed(4)
+    S, K, N = 37, 528, 96
+    x = _rows(g, S, K, torch.bfloat16)
+    q, s = R.weights(g, 1, N, K)
+    q, s = q[0].to(DEV), s[0].to(DEV)
+    want = fp8.linear(x.to(DEV), q, s)
+    for pad, off in ((8, 0), (16, 8), (5, 1)):
+        xb = torch.full((S, K + pad + off), float("nan"), dtype=torch.bfloat16, device=DEV)
+        xb[:, off:off + K] = x.to(DEV)
+        assert torch.equal(fp8.linear(xb[:, off:off + K], q, s), want)
+    rows = fp8.quantize_rows(x.to(DEV))
+    dense = fp8.Fp8Rows(rows.q, rows.scale.view(torch.uint8).contiguous().view(R.E8M0))     # 5 scales a row: re-laid
+    assert torch.equal(fp8.linear(dense, q, s), want)
+    wide = torch.zeros((S, K + 48), dtype=torch.uint8, device=DEV)
+    wide[:, 16:16 + K] = rows.q.view(torch.uint8)
+    assert torch.equal(fp8.linear(fp8.Fp8Rows(wide.view(R.E4M3)[:, 16:16 + K], rows.scale), q, s), want)
+    odd = torch.zeros(N * 2 + 3, dtype=torch.bfloat16, device=DEV)[3:3 + N]                  # a bias at an odd address
+    odd.copy_(torch.randn(N, generator=g))
+    assert torch.equal(fp8.linear(x.to(DEV), q, s, odd), fp8.linear(x.to(DEV), q, s, odd.clone()))
+    assert tuple(fp8.linear(x.to(DEV).view(37, 1, 1, K), q, s).shape) == (37, 1, 1, N)
+    assert tuple(fp8.linear(x.to(DEV)[:0], q, s).shape) == (0, N)
+    assert tuple(fp8.linear(x.to(DEV)[0], q, s).shape) == (N,)
+
+
+def test_non_finite_rows_stay_in_their_rows():
+    g = torch.Generator().manual_seed(8)
+    x = _rows(g, 40, 384, torch.bfloat16)
+    q, s = R.weights(g, 1, 80, 384)
+    clean = fp8.linear(x.to(DEV), q[0].to(DEV), s[0].to(DEV))
+    x[3, 200] = float("inf")
+    x[17, 0] = float("nan")
+    y = fp8.linear(x.to(DEV), q[0].to(DEV), s[0].to(DEV))
+    bad = torch.zeros(40, dtype=torch.bool)
+    bad[[3, 17]] = True
+    assert bool(torch.isnan(y[bad.to(DEV)]).all()) and torch.equal(y[~bad.to(DEV)], clean[~bad.to(DEV)])
+
+
+# ------------------------------------------------------------------------------------------------ expert MLP
+def _act(a, I, act, n_gated):
+    if act == "swiglu":
+        u, v = a[:, :I], a[:, I:]
+        gate = u * torch.sigmoid(u)
+        if 0 <= n_gated < I:
+            gate = torch.where(torch.arange(I) < n_gated, gate, torch.ones((), dtype=D))
+        return gate * v
+    return 0.5 * a * (1 + torch.tanh((2 / torch.pi) ** 0.5 * (a + 0.044715 * a ** 3)))
+
+
+def _ffn_ref(x, q1, s1, q2, s2, b1, b2, act, n_gated=-1):
+    """y and its bound for one expert's rows.  The first product is off by at most `t1` (_fp8_ref), which moves the
+    activation by at most its slope (|silu'| < 1.1, |gelu'| < 1.13) times that, + 2^-20 of its terms for fp32 exp and
+    reciprocal.  Quantisation is monotone for a given scale, so every hidden value lies between those of h - d and h + d,
+    with the scale that the block's maximum may have at either end."""
+    I = q2.shape[1]
+    parts = 2 if act == "swiglu" else 1
+    a, t1 = R.product(R.deq(x), R.deq_stored(q1, s1, parts))
+    if b1 is not None:
+        a = a + b1.to(D)
+    h = _act(a, I, act, n_gated)
+    if act == "swiglu":
+        u, v = a[:, :I], a[:, I:]
+        tu, tv = t1[:, :I], t1[:, I:]
+        gate = _act(torch.cat([u, torch.ones_like(u)], 1), I, act, n_gated)
+        d = 1.1 * tu * (v.abs() + tv) + gate.abs() * tv + 2.0 ** -20 * (u.abs() * v.abs() + h.abs())
+    else:
+        d = 1.13 * t1 + 2.0 ** -20 * a.abs()
+    top = R._top(h)
+    e = R._top(d)                                   # the block's maximum moves by at most its largest d
+    mid = R.deq(h)
+    dev = torch.zeros_like(h)
+    for b in (R.scale_byte((top - e).clamp_min(0)), R.scale_byte(top + e)):
+        sc = R.spread(torch.exp2(b.to(D) - 127), *h.shape)
+        lim = 448.0
+        for v in (h - d, h + d):
+            dev = torch.maximum(dev, (R.e4m3((v / sc).clamp(-lim, lim)) * sc - mid).abs())
+    w2 = R.deq_stored(q2, s2)
+    y, t2 = R.product(mid, w2)
+    if b2 is not None:
+        y = y + b2.to(D)
+    return y, t2 + (1 + 2.0 ** -9) * (dev @ w2.abs().t())
+
+
+def _check_ffn(y, ref, tol):
+    g = y.cpu().to(D)
+    h = R.half_step(y.dtype)
+    lim = tol + h * (ref.abs() + tol) + 2.0 ** -25
+    assert bool(((g - ref).abs() <= lim).all()), float(((g - ref).abs() / lim).max())
+    # by norm: the first product's truncations (2^-11 of its size at most) move that share of a step's width of the hidden
+    # values, 2^-11 / 2^-4 < 1 %, by one step (2^-3 at most): sqrt(0.01) * 2^-3 = 2^-6.3; together with half a step of y
+    rel = float((g - ref).norm() / ref.norm().clamp_min(1e-30))
+    assert rel <= h + 2.0 ** -6.3, rel
+
+
+FFN = [("swiglu", 2, 1, 64, 128), ("swiglu", 4, 3, 256, 384), ("swiglu", 4, 30, 272, 144), ("gelu_new", 4, 17, 128, 272),
+       ("swiglu", 8, 200, 128, 176), ("gelu_new", 2, 150, 144, 640), ("swiglu", 4, 600, 640, 256), ("gelu_new", 3, 333, 400, 528),
+       ("swiglu", 2, 64, 2048, 512), ("swiglu", 4, 32, 512, 2064), ("gelu_new", 4, 33, 2560, 256)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act,E,S,M,I", FFN)
+def test_expert_ffn(act, E, S, M, I, dt):
+    g = torch.Generator().manual_seed(S + M + I)
+    parts = 2 if act == "swiglu" else 1
+    x = _rows(g, S, M, dt)
+    q1, s1 = R.weights(g, E, I, M, parts)
+    q2, s2 = R.weights(g, E, M, I)
+    bias = act == "gelu_new" or S == 200
+    b1 = torch.randn((E, parts * I), generator=g).to(dt) if bias else None
+    b2 = torch.randn((E, M), generator=g).to(dt) if bias else None
+    two = torch.stack([torch.randperm(E, generator=g)[:2] for _ in range(S)])
+    if E > 2:
+        two[two == 1] = 0                           # expert 1 gets nothing (a token may then name an expert twice)
+    two = two.reshape(-1)
+    perm = torch.sort(two, stable=True).indices
+    offs = torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(two, minlength=E).cumsum(0)])
+    n_gated = I // 3 if (act == "swiglu" and S == 30) else -1
+    gpu = [t.to(DEV) if t is not None else None for t in (q1, s1, q2, s2, b1, b2)]
+    kw = dict(gather=perm.to(torch.int32).to(DEV), gather_shift=1, b1=gpu[4], b2=gpu[5], n_gated=n_gated)
+    po = offs.to(torch.int32).to(DEV)
+    y = fp8.expert_ffn(act, x.to(DEV), *gpu[:4], po, 2 * S, **kw)
+    ref, tol = torch.empty((2 * S, M), dtype=D), torch.empty((2 * S, M), dtype=D)
+    for e in range(E):
+        a, b = int(offs[e]), int(offs[e + 1])
+        if b > a:
+            ref[a:b], tol[a:b] = _ffn_ref(x[perm[a:b] >> 1], q1[e], s1[e], q2[e], s2[e], b1[e] if bias else None,
+                                          b2[e] if bias else None, act, n_gated)
+    _check_ffn(y, ref, tol)
+    y2 = fp8.expert_ffn(act, fp8.quantize_rows(x.to(DEV)), *gpu[:4], po, 2 * S, out_dtype=dt, **kw)
+    assert torch.equal(y, y2)                       # 8-bit rows, same bits
+    assert torch.equal(y, fp8.expert_ffn(act, x.to(DEV), *gpu[:4], po, 2 * S, **kw))
+
+
+def test_expert_ffn_leaves_other_rows_alone():
+    g = torch.Generator().manual_seed(3)
+    E, M, I = 2, 128, 256
+    q1, s1 = R.weights(g, E, I, M, 2)
+    q2, s2 = R.weights(g, E, M, I)
+    for rows, lead, used in ((100, 0, 60), (40, 3, 20), (300, 0, 0), (600, 10, 500)):
+        x = _rows(g, rows, M, torch.bfloat16).to(DEV)
+        offs = torch.tensor([lead, lead + used // 3, lead + used], dtype=torch.int32, device=DEV)
+        # through the C entry, so that the output holds a known pattern before the call
+        lib = _lib.load()
+        y = torch.full((rows, M), 7.0, dtype=torch.bfloat16, device=DEV)
+        n = lib.moe_expert_ffn_fp8_workspace_bytes(rows, rows, M, I)
+        guard = 4096
+        ws = torch.full((n + guard,), 0x5A, dtype=torch.uint8, device=DEV)
+        t = [v.to(DEV) for v in (q1, s1, q2, s2)]
+        rc = lib.moe_expert_ffn_fp8_fwd(0, x.data_ptr(), M, rows, None, 0, None, 0, None, 0, t[0].data_ptr(), t[1].data_ptr(),
+                                        None, t[2].data_ptr(), t[3].data_ptr(), None, offs.data_ptr(), E, E, rows, M, I, -1,
+                                        ws.data_ptr(), n, y.data_ptr(), 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert bool((y[:lead] == 7).all()) and bool((y[lead + used:] == 7).all())
+        assert bool((ws[n:] == 0x5A).all())
+        if used:
+            ref = torch.cat([_ffn_ref(x.cpu()[a:b], q1[e], s1[e], q2[e], s2[e], None, None, "swiglu")[0]
+                             for e, (a, b) in enumerate(((lead, lead + used // 3), (lead + used // 3, lead + used)))])
+            assert float((y[lead:lead + used].cpu().to(D) - ref).norm() / ref.norm()) <= 2.0 ** -6
+
+
+def test_norm_and_ffn_together_and_in_a_graph():
+    """The order of a decoder layer: norm with 8-bit output, then the expert MLP on those rows; eager, on a side stream, and
+    captured twice (two graphs with workspaces of their own), replayed alternately with eager work between."""
+    g = torch.Generator().manual_seed(12)
+    E, M, I, S = 4, 256, 512, 24
+    q1, s1 = (t.to(DEV) for t in R.weights(g, E, I, M, 2))
+    q2, s2 = (t.to(DEV) for t in R.weights(g, E, M, I))
+    w = torch.ones(M, dtype=torch.bfloat16, device=DEV)
+    perm = torch.arange(2 * S, dtype=torch.int32, device=DEV)
+    offs = torch.tensor([0, 10, 11, 40, 48], dtype=torch.int32, device=DEV)
+
+    def layer(x, r):
+        rows, y, s = norm.add_rms_norm_fp8(x, r, w)
+        return fp8.expert_ffn("swiglu", rows, q1, s1, q2, s2, offs, 2 * S, perm, 1), s
+
+    xs = [_rows(g, S, M, torch.bfloat16).to(DEV) for _ in range(2)]
+    r = _rows(g, S, M, torch.bfloat16).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = layer(xs[0], r)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(on_side[0], layer(xs[0], r)[0])
+    ins = [x.clone() for x in xs]
+    graphs, outs = [], []
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(layer(ins[i], r))
+        graphs.append(gr)
+    for k in range(4):
+        new = [(x.float() * (1 + k)).to(torch.bfloat16) for x in xs]
+        for i in range(2):
+            ins[i].copy_(new[i])
+        graphs[0].replay()
+        graphs[1].replay()
+        eager = [layer(n, r) for n in new]
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i][0], eager[i][0]) and torch.equal(outs[i][1], eager[i][1])
+
+
+def test_gradient_captured_while_an_eager_graph_lives():
+    g = torch.Generator().manual_seed(2)
+    q, s = R.weights(g, 1, 128, 256)
+    q, s = q[0].to(DEV), s[0].to(DEV)
+    x = _rows(g, 20, 256, torch.bfloat16).to(DEV)
+    dy = _rows(g, 20, 128, torch.bfloat16).to(DEV)
+    xe = x.clone().requires_grad_(True)
+    want, = torch.autograd.grad(fp8.linear(xe, q, s), xe, dy)
+    xc = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        leaf = xc.detach().requires_grad_(True)     # a leaf of the captured pass: no eager node refers to it
+        got, = torch.autograd.grad(fp8.linear(leaf, q, s), leaf, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_refusals_on_the_gpu():
+    g = torch.Generator().manual_seed(1)
+    q, s = (t.to(DEV) for t in R.weights(g, 2, 64, 128))
+    x = _rows(g, 8, 128, torch.bfloat16).to(DEV)
+    offs = torch.tensor([0, 4, 8], dtype=torch.int32, device=DEV)
+    for bad in (lambda: fp8.linear(x[:, :64], q[0], s[0]), lambda: fp8.linear(x, q[0], s[0, :, :0]),
+                lambda: fp8.linear(x, q[0][:, ::2], s[0]), lambda: fp8.linear(x, q, s),
+                lambda: fp8.grouped_linear(x, q, s, offs.long()), lambda: fp8.grouped_linear(x, q, s, offs.cpu()),
+                lambda: fp8.grouped_linear(x, q, s, offs[:1]), lambda: fp8.linear(x, q[0], s[0], torch.zeros(64, device=DEV)),
+                lambda: fp8.quantize_rows(x[:, :40]), lambda: fp8.quantize_weight(x[:, :40]),
+                lambda: fp8.linear(x.float(), q[0], s[0]), lambda: fp8.linear(x, q[0].float(), s[0]),
+                lambda: fp8.linear(x, q[0], s[0].view(torch.uint8)), lambda: fp8.linear(x.cpu(), q[0], s[0]),
+                lambda: fp8.linear(x, q[0], s[0], out_dtype=torch.float16),
+                lambda: fp8.linear(fp8.quantize_rows(x), q[0], s[0], out_dtype=torch.float32)):
+        with pytest.raises((ValueError, TypeError, _lib.MoEKernelError)):
+            bad()
+    with pytest.raises(NotImplementedError):
+        fp8.linear(x, q[0], s[0], torch.zeros(64, dtype=torch.bfloat16, device=DEV, requires_grad=True))
+    qo, so = (t.to(DEV) for t in R.weights(g, 1, 50, 128))
+    with pytest.raises(NotImplementedError):
+        fp8.linear(x.clone().requires_grad_(True), qo[0], so[0])        # 50 output columns: no 16-byte rows of the gradient
+    q1, s1 = (t.to(DEV) for t in R.weights(g, 2, 32, 128, 2))
+    q2, s2 = (t.to(DEV) for t in R.weights(g, 2, 128, 32))
+    fp8.expert_ffn("swiglu", x, q1, s1, q2, s2, offs, 8)
+    for bad in (lambda: fp8.expert_ffn("relu", x, q1, s1, q2, s2, offs, 8), lambda: fp8.expert_ffn("gelu_new", x, q1, s1, q2, s2, offs, 8),
+                lambda: fp8.expert_ffn("swiglu", x, q1, s1, q2, s2, offs, 9), lambda: fp8.expert_ffn("swiglu", x, q1, s1[:, :1], q2, s2, offs, 8),
+                lambda: fp8.expert_ffn("swiglu", x, q1, s1, q2, s2, offs, 8, gather=offs),
+                lambda: fp8.expert_ffn("swiglu", x.half(), q1, s1, q2, s2, offs, 8, b2=torch.zeros((2, 128), dtype=torch.bfloat16, device=DEV))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        fp8.expert_ffn("swiglu", x.clone().requires_grad_(True), q1, s1, q2, s2, offs, 8)
