@@ -11,6 +11,11 @@
 
 namespace moe {
 
+typedef unsigned char u8;
+typedef __attribute__((ext_vector_type(8))) int v8i_t;
+typedef __attribute__((ext_vector_type(4))) int v4i_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+
 constexpr int QB = 128;               // elements that share a scale along K (and weight rows along N)
 constexpr unsigned E8M0_NAN = 255u;   // scale of a block that holds an infinity or a NaN; its elements are all NaN
 
@@ -37,5 +42,50 @@ __device__ __forceinline__ unsigned umax_xor(unsigned v, int mask) {
     const unsigned o = (unsigned)__shfl_xor((int)v, mask, 64);
     return v > o ? v : o;
 }
+
+// activations in fp32 (nothing is rounded between the accumulator and the quantisation: a 16-bit rounding there would move
+// ~1 % of the elements to a neighbouring e4m3 value)
+__device__ __forceinline__ float gelu_new_f32(float x) {
+    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
+    // 0.5 x (1 + tanh u) = x / (1 + exp(-2u))
+    return x * __builtin_amdgcn_rcpf(1.f + __expf(-2.f * u));
+}
+
+struct Fp8GemmParams {
+    const u8 *a;              // rows, e4m3, row stride lda bytes
+    long long lda;
+    const u8 *a_scale;        // e8m0 [rows, ceil(K/128)], row stride lds_a bytes (a multiple of 4, rows 4-byte aligned)
+    long long ld_as;
+    const int *gather;
+    int gather_shift;
+    const u8 *w;              // [experts, N (or 2N), K]
+    long long w_expert_stride;
+    const u8 *w_scale;        // [experts, blocks of N (or 2x), ceil(K/128)], dense
+    long long ws_expert_stride;
+    const bf16_t *bias;
+    long long bias_expert_stride;
+    const int *group_offsets; // NULL: one group, rows [0, max_rows)
+    int G, n_experts, max_rows;
+    void *out;                // 16-bit [rows, ldo], or e4m3 with out_scale
+    long long ldo;
+    u8 *out_scale;            // [rows, ceil(N/128)], row stride ld_os
+    long long ld_os;
+    int K, N_out;
+    int b_row_offset;         // gated: weight row of the first 'b' projection row (= N_out)
+    int b_blk_offset;         // gated: row of the scales' grid where the 'b' projection starts
+    int n_gated;
+    int col_tiles, rs;
+    int vec_store;            // 16-bit output: rows and pointer allow 16-byte stores
+    int zero_tail;            // 16-bit output: rows of [0, max_rows) that belong to no group are set to 0
+    const bf16_t *x16;        // few-row launches: 16-bit rows (row stride ldx elements) quantised on load; a, a_scale unused
+    long long ldx;
+    float *h32;               // few-row launches of a first product: fp32 activations [rows, N_out], quantised by a launch behind
+    int dtype;
+};
+
+// Launches of few rows (moe_fp8_gemv.hip): at most FP8_FEW_ROWS of them in all.
+constexpr int FP8_FEW_ROWS = 64;
+int launch_fp8_few(const Fp8GemmParams &p, int epilogue, hipStream_t st);
+int launch_quantize_f32(const float *h, int rows, int I, u8 *q, u8 *scale, long long ld_scale, hipStream_t st);
 
 }  // namespace moe

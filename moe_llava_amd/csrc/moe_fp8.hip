@@ -18,38 +18,7 @@
 
 namespace moe {
 
-typedef __attribute__((ext_vector_type(8))) int v8i_t;
-typedef __attribute__((ext_vector_type(4))) int v4i_t;
-typedef __attribute__((ext_vector_type(4))) float f32x4_t;
-typedef unsigned char u8;
 
-struct Fp8GemmParams {
-    const u8 *a;              // rows, e4m3, row stride lda bytes
-    long long lda;
-    const u8 *a_scale;        // e8m0 [rows, ceil(K/128)], row stride lds_a bytes (a multiple of 4, rows 4-byte aligned)
-    long long ld_as;
-    const int *gather;
-    int gather_shift;
-    const u8 *w;              // [experts, N (or 2N), K]
-    long long w_expert_stride;
-    const u8 *w_scale;        // [experts, blocks of N (or 2x), ceil(K/128)], dense
-    long long ws_expert_stride;
-    const bf16_t *bias;
-    long long bias_expert_stride;
-    const int *group_offsets; // NULL: one group, rows [0, max_rows)
-    int G, n_experts, max_rows;
-    void *out;                // 16-bit [rows, ldo], or e4m3 with out_scale
-    long long ldo;
-    u8 *out_scale;            // [rows, ceil(N/128)], row stride ld_os
-    long long ld_os;
-    int K, N_out;
-    int b_row_offset;         // gated: weight row of the first 'b' projection row (= N_out)
-    int b_blk_offset;         // gated: row of the scales' grid where the 'b' projection starts
-    int n_gated;
-    int col_tiles, rs;
-    int vec_store;            // 16-bit output: rows and pointer allow 16-byte stores
-    int zero_tail;            // 16-bit output: rows of [0, max_rows) that belong to no group are set to 0
-};
 
 constexpr int FTHREADS = 512;
 constexpr int FLW = 4;                 // loader waves (one per SIMD)
@@ -95,14 +64,6 @@ struct FTile {
     static constexpr int NF = BNW / 64;                       // 16-row weight fragments per wave
     static constexpr int WNT = BNW / 4;                       // weight rows per wave
 };
-
-// activations in fp32 (nothing is rounded between the accumulator and the quantisation: a 16-bit rounding there would move
-// ~1 % of the elements to a neighbouring e4m3 value)
-__device__ __forceinline__ float gelu_new_f32(float x) {
-    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
-    // 0.5 x (1 + tanh u) = x / (1 + exp(-2u))
-    return x * __builtin_amdgcn_rcpf(1.f + __expf(-2.f * u));
-}
 
 template <int DT, int EPI, int BM, int BNW>
 __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmParams p) {
@@ -463,8 +424,12 @@ static int launch_fp8_gemm(const Fp8GemmParams &p, hipStream_t st) {
     return launch_fp8_tile<DT, EPI, 32, 256>(p, st);
 }
 
-static int fp8_gemm(const Fp8GemmParams &p, int epilogue, int dtype, hipStream_t st) {
+static int fp8_gemm(Fp8GemmParams p, int epilogue, int dtype, hipStream_t st) {
+    p.dtype = dtype;
     if (p.max_rows == 0) return 0;
+    // a few rows stream the weights: no tile of the ring kernel has enough blocks for that (32 x 256 tiles at two active
+    // experts: 88 blocks for 256 CUs).  The few-row kernel has no rows to clear: zero_tail launches stay on the tiles.
+    if (p.max_rows <= FP8_FEW_ROWS && !p.zero_tail && (epilogue == MOE_EPI_PLAIN || p.h32)) return launch_fp8_few(p, epilogue, st);
 #define FP8_EPI(DT_)                                                                   \
     switch (epilogue) {                                                                \
         case MOE_EPI_SWIGLU: return launch_fp8_gemm<DT_, EPI_SWIGLU>(p, st);           \
@@ -525,6 +490,7 @@ namespace {
 inline size_t pad256b(size_t b) { return (b + 255) & ~(size_t)255; }
 struct FfnWs {
     u8 *hq, *hs, *aq, *as;
+    float *h32;
     long long ld_hs, ld_as;
     size_t total;
 };
@@ -537,8 +503,10 @@ FfnWs carve_ffn(void *ws, int src_rows, int max_rows, int M, int I) {
     r.ld_as = ((M + QB - 1) / QB + 3) / 4 * 4;
     r.hq = take((size_t)max_rows * I);
     r.hs = take((size_t)max_rows * r.ld_hs);
+    const bool few = max_rows <= FP8_FEW_ROWS;  // the activation leaves the first product in fp32
     r.aq = take((size_t)src_rows * M);
     r.as = take((size_t)src_rows * r.ld_as);
+    r.h32 = (float *)take(few ? (size_t)max_rows * I * 4 : 0);
     r.total = off;
     return r;
 }
@@ -565,13 +533,20 @@ extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int s
     if (!aligned16(workspace) || !aligned16(y)) return fail(MOE_ERR_ALIGN, "%s: workspace and y must be 16-byte aligned", fn);
     const FfnWs ws = carve_ffn(workspace, x ? src_rows : 0, max_rows, M, I);
     if (ws_bytes < ws.total) return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, ws_bytes, ws.total);
-    if (x) { a = max_rows ? ws.aq : workspace; lda = M; a_scale = max_rows ? ws.as : workspace; ld_as = ws.ld_as; }
+    const bool few = max_rows <= FP8_FEW_ROWS;
+    if (x) {
+        if (src_rows > 1 && ldx < M) return fail(MOE_ERR_SHAPE, "%s: row stride %lld < M", fn, (long long)ldx);
+        if (reinterpret_cast<uintptr_t>(x) & 1) return fail(MOE_ERR_ALIGN, "%s: x must be 2-byte aligned", fn);
+        a = max_rows ? ws.aq : workspace; lda = M; a_scale = max_rows ? ws.as : workspace; ld_as = ws.ld_as;
+    }
     int rc = fp8_args_ok(fn, a, lda, a_scale, ld_as, gather_shift, w1, w1_scale, b1, G, n_experts_local, max_rows, M, I);
     if (rc) return rc;
     rc = fp8_args_ok(fn, workspace, I, workspace, ws.ld_hs, 0, w2, w2_scale, b2, G, n_experts_local, max_rows, I, M);
     if (rc) return rc;
     if (max_rows == 0) return 0;
-    if (x && (rc = moe_quantize_rows_fp8(x, ldx, src_rows, M, ws.aq, M, ws.as, ws.ld_as, dtype, stream))) return rc;
+    // few rows: quantised on load, when wide loads can fetch them
+    const bool on_load = x && few && aligned16(x) && (ldx & 7) == 0;
+    if (x && !on_load && (rc = moe_quantize_rows_fp8(x, ldx, src_rows, M, ws.aq, M, ws.as, ws.ld_as, dtype, stream))) return rc;
     const bool gated = act == MOE_ACT_SWIGLU;
     const int mb = (M + QB - 1) / QB, ib = (I + QB - 1) / QB;
     Fp8GemmParams p{};
@@ -584,7 +559,9 @@ extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int s
     p.out = ws.hq; p.ldo = I; p.out_scale = ws.hs; p.ld_os = ws.ld_hs;
     p.K = M; p.N_out = I; p.b_row_offset = I; p.b_blk_offset = ib;
     p.n_gated = (n_gated < 0 || n_gated > I) ? I : n_gated;
+    if (few) { p.x16 = on_load ? (const bf16_t *)x : nullptr; p.ldx = ldx; p.h32 = ws.h32; }
     if ((rc = fp8_gemm(p, gated ? MOE_EPI_SWIGLU : MOE_EPI_GELU_NEW, dtype, (hipStream_t)stream))) return rc;
+    if (few && (rc = launch_quantize_f32(ws.h32, max_rows, I, ws.hq, ws.hs, ws.ld_hs, (hipStream_t)stream))) return rc;
     return moe_grouped_gemm_fp8_fwd(ws.hq, I, ws.hs, ws.ld_hs, nullptr, 0, w2, w2_scale, b2, group_offsets, G, n_experts_local,
                                     max_rows, I, M, 0, y, M, dtype, stream);
 }

@@ -14,8 +14,6 @@
 
 namespace moe {
 
-typedef unsigned char u8;
-
 struct NormParams {
     const bf16_t *x, *res;
     long long ldx, ldr;
