@@ -365,7 +365,9 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
         __syncthreads();
     };
     constexpr int TF = BM / 16;
-    constexpr int AMF = TF / 2;
+    // 256 x 256: the loader waves own 5 of the 16 row fragments, their SIMD partners 11: a loader wave spends the head of a
+    // slice issuing its fills.  Measured (45056 rows, K 5632, N 2048): 473 -> 457 us; 6, 7 within 1 % of 8.
+    constexpr int AMF = BM == 256 && BNW == 256 ? 5 : TF / 2;
     if (wave < FLW) {
         setup_ptrs();
         tile_body(FInt<AMF>{}, FInt<1>{}, 0);
@@ -373,7 +375,19 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
         tile_body(FInt<TF - AMF>{}, FInt<0>{}, AMF * 16);
     }
 
-    // ---- image -> global, 16 bytes a lane ----
+    // ---- image -> global, 16 bytes a lane; 2 bytes a lane (consecutive lanes, consecutive columns) where the output's rows
+    //      do not allow that (8 scattered 2-byte stores a lane took 13 us of a 29.5-us launch, 333 rows, K 1008, N 1003) ----
+    typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+    if (!T::QOUT && !p.vec_store) {
+        const int rows = min(BM, row_end - row_begin), cols = min(NC, p.N_out - ct * NC);
+        constexpr int RPI = FTHREADS / 64;
+        for (int r = wave; r < rows; r += RPI)
+#pragma unroll
+            for (int c = lane; c < NC; c += 64)
+                if (c < cols)
+                    ((bf16_t *)p.out)[(long long)(row_begin + r) * p.ldo + ct * NC + c] = *reinterpret_cast<const bf16_t *>(lds + r * ROWB + c * 2);
+        return;
+    }
     constexpr int EL = T::QOUT ? 16 : 8;  // elements per 16-byte chunk
     constexpr int CPR = NC / EL, RPI = FTHREADS / CPR;
     const int cc = tid % CPR, r0 = tid / CPR;
@@ -384,13 +398,12 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
     for (int r = r0; r < BM; r += RPI) {
         const int prow = row_begin + r;
         if (prow >= row_end) break;
-        typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
         const u32x4_t v = *reinterpret_cast<const u32x4_t *>(lds + r * ROWB + cc * 16);
         if constexpr (T::QOUT) {
             __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t *>((u8 *)p.out + (long long)prow * p.ldo + col));
         } else {
             bf16_t *dst = (bf16_t *)p.out + (long long)prow * p.ldo + col;
-            if (left >= 8 && p.vec_store) {
+            if (left >= 8) {
                 __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t *>(dst));
             } else {
 #pragma unroll
@@ -413,15 +426,59 @@ static int launch_fp8_tile(Fp8GemmParams p, hipStream_t st) {
     return check_launch("fp8_gemm_kernel");
 }
 
+// Tile choice.  One block runs on a CU at a time, so a launch takes ceil(tiles / 256) rounds of (slices * step + fixed);
+// a launch of many rounds is held by the fills instead, tiles * slices * (BM + BNW) * 128 bytes at ~10.5 TB/s from L2.  The
+// constants were measured on one-round launches (K = 5632 and 10240, one group and four; microseconds): they are a CU's time
+// per slice with its fills in flight, and prologue + epilogue.  The smallest estimate is within 5 % of the best of
+// twelve tiles on 36 of 40 swept shapes (100 ... 11264 rows, K 1024 ... 10240, N 1024 ... 5632, 1 to 8 groups) and 21 % off
+// at worst; the 256 x 256 tile alone is up to 3.2 x off there (1408 rows, K 5632, N 2048, 4 groups: 57.9 us against 30.9).
+struct Fp8Tile { int bm, bn; float step, fixed; };
+constexpr Fp8Tile FP8_TILES[] = {{256, 256, 1.15f, 6.5f}, {128, 256, 0.86f, 5.0f}, {256, 128, 0.85f, 5.0f}, {128, 128, 0.54f, 5.5f},
+                                 {64, 256, 0.63f, 4.5f},  {64, 128, 0.40f, 5.5f},  {32, 256, 0.54f, 3.0f},  {32, 128, 0.38f, 5.0f},
+                                 {32, 64, 0.31f, 5.0f}};
+template <int EPI>
+static bool fp8_tile_ok(int bm, int bn, int kq) {
+    if (bm * kq > FP8_STRIP) return false;                     // the tile's scales have to fit their LDS
+    if (EPI == EPI_SWIGLU) return bn == 256;                   // 128 output columns = one block of the quantisation
+    if (EPI == EPI_GELU_NEW) return bn == 256 || bn == 128;
+    return true;
+}
+template <int EPI>
+static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p) {
+    const int nk = (p.K + QB - 1) / QB, kq = (nk + 3) / 4 * 4;
+    const double parts = p.max_rows < p.G ? p.max_rows : p.G;  // groups that can hold rows: half a tile of each is lost
+    const Fp8Tile *best = nullptr;
+    double best_t = 0;
+    for (const Fp8Tile &t : FP8_TILES) {
+        if (!fp8_tile_ok<EPI>(t.bm, t.bn, kq)) continue;
+        const int nc = EPI == EPI_SWIGLU ? t.bn / 2 : t.bn;
+        const double rt = p.G == 1 ? (double)((p.max_rows + t.bm - 1) / t.bm) : ((double)p.max_rows / t.bm + 0.5 * parts) * 1.05;
+        const double tiles = rt * ((p.N_out + nc - 1) / nc);
+        const double rounds = (double)(long long)((tiles + 255) / 256);
+        const double fill = tiles * nk * (t.bm + t.bn) * 128e-6 / 10.5;
+        double us = rounds * (nk * t.step + t.fixed);
+        if (fill > us) us = fill;
+        if (!best || us < best_t) { best = &t; best_t = us; }
+    }
+    return *best;
+}
+
 template <int DT, int EPI>
 static int launch_fp8_gemm(const Fp8GemmParams &p, hipStream_t st) {
-    const int kq = ((p.K + QB - 1) / QB + 3) / 4 * 4;
-    const long long per = (p.max_rows + p.G - 1) / p.G;  // rows of an average group
-    const bool fits256 = 256 * kq <= FP8_STRIP, fits128 = 128 * kq <= FP8_STRIP, fits64 = 64 * kq <= FP8_STRIP;
-    if (per > 192 && fits256) return launch_fp8_tile<DT, EPI, 256, 256>(p, st);
-    if (per > 64 && fits128) return launch_fp8_tile<DT, EPI, 128, 256>(p, st);
-    if (per > 32 && fits64) return launch_fp8_tile<DT, EPI, 64, 256>(p, st);
-    return launch_fp8_tile<DT, EPI, 32, 256>(p, st);
+    int bm, bn;
+    const Knobs &k = knobs();
+    if (k.tile_bm && fp8_tile_ok<EPI>(k.tile_bm, k.tile_bnw, ((p.K + QB - 1) / QB + 3) / 4 * 4)) {
+        bm = k.tile_bm; bn = k.tile_bnw;
+    } else {
+        const Fp8Tile &t = choose_fp8_tile<EPI>(p);
+        bm = t.bm; bn = t.bn;
+    }
+#define FP8_TILE(M_, N_) if (bm == M_ && bn == N_) return launch_fp8_tile<DT, EPI, M_, N_>(p, st);
+    FP8_TILE(256, 256) FP8_TILE(128, 256) FP8_TILE(64, 256) FP8_TILE(32, 256)
+    if constexpr (EPI != EPI_SWIGLU) { FP8_TILE(256, 128) FP8_TILE(128, 128) FP8_TILE(64, 128) FP8_TILE(32, 128) }
+    if constexpr (EPI == EPI_PLAIN) { FP8_TILE(32, 64) }
+#undef FP8_TILE
+    return fail(MOE_ERR_ARG, "fp8 product: no tile %d x %d", bm, bn);
 }
 
 static int fp8_gemm(Fp8GemmParams p, int epilogue, int dtype, hipStream_t st) {

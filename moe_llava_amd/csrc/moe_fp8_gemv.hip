@@ -13,6 +13,12 @@
 
 namespace moe {
 
+#ifndef FEW_FRAGS
+#define FEW_FRAGS 8
+#endif
+#ifndef FEW_KS
+#define FEW_KS 8
+#endif
 template <int N>
 struct FewInt { static constexpr int value = N; };
 
@@ -21,7 +27,7 @@ struct FewCfg {
     static constexpr bool GATED = EPI == EPI_SWIGLU;
     static constexpr int NACC = GATED ? 2 : 1;
     static constexpr int COLS = 16 * NW;
-    static constexpr int U = 4 / (NACC * NW);  // blocks of K in flight: 4 fragments = 8 weight loads of 1 KiB per wave
+    static constexpr int U = FEW_FRAGS / (NACC * NW) > 1 ? FEW_FRAGS / (NACC * NW) : 1;
 };
 
 template <int DT, int EPI, int NW, bool X16, int RT>
@@ -126,9 +132,11 @@ __device__ __forceinline__ void few_body(const Fp8GemmParams &p, int expert, int
 #pragma unroll
                     for (int g = 0; g < NW; ++g) fw[u][h][g] = ldw(wr[h][g], kb + u, last);
 #pragma unroll
-            for (int u = 0; u < UU; ++u) {
+            for (int u = 0; u < UU; ++u)
 #pragma unroll
                 for (int t = 0; t < RT; ++t) fx[u][t] = ldx(t, kb + u, last);
+#pragma unroll
+            for (int u = 0; u < UU; ++u) {
 #pragma unroll
                 for (int h = 0; h < NACC; ++h) {
                     const int ws = __builtin_amdgcn_readlane(wsc[h], kb + u - k0);
@@ -255,7 +263,7 @@ int launch_fp8_few(const Fp8GemmParams &p0, int epilogue, hipStream_t st) {
     if (grid > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "fp8 product: grid too large");
     // waves per block: about 16 wave-tasks per CU, at least one block of K each
     const int nk = (p.K + QB - 1) / QB;
-    int ks = 8;
+    int ks = FEW_KS;
     while (ks > 1 && (active * p.col_tiles * ks > 4096 || ks > nk)) ks >>= 1;
     const dim3 g((unsigned)grid), b(64 * ks);
 #define FEW(E_, N_, X_)                                                                                        \
