@@ -400,6 +400,14 @@ int moe_grouped_gemm_fp8_fwd(const void *a, int64_t lda, const void *a_scale, in
                              const int32_t *group_offsets, int G, int n_experts_local, int max_rows, int K, int N,
                              int zero_tail, void *out, int64_t ldo, int dtype, void *stream);
 
+/* moe_grouped_linear_fp8_fwd: moe_grouped_gemm_fp8_fwd on 16-bit rows x [rows, K] (row stride ldx elements, any alignment),
+ * quantised as moe_quantize_rows_fp8 would, into the workspace or on load.  Workspace contents mean nothing between calls;
+ * calls that may overlap need one each. */
+size_t moe_grouped_linear_fp8_workspace_bytes(int rows, int K);
+int moe_grouped_linear_fp8_fwd(const void *x, int64_t ldx, const void *w, const void *w_scale, const void *bias,
+                               const int32_t *group_offsets, int G, int n_experts_local, int rows, int K, int N, int zero_tail,
+                               void *workspace, size_t ws_bytes, void *out, int64_t ldo, int dtype, void *stream);
+
 /* moe_expert_ffn_fp8_fwd: moe_expert_ffn_fwd on 8-bit experts.  Activation in fp32 on the accumulators (no 16-bit rounding
  * between the products), quantised per 1 x 128 block of the I hidden channels for the second product.
  *   x [src_rows, M] 16-bit rows (quantised into the workspace), or NULL and a / a_scale: rows that are 8-bit already

@@ -94,6 +94,10 @@ _SIGNATURES = [
     ("moe_grouped_gemm_fp8_fwd", c_int,
      [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
       c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p]),
+    ("moe_grouped_linear_fp8_workspace_bytes", c_size_t, [c_int, c_int]),
+    ("moe_grouped_linear_fp8_fwd", c_int,
+     [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t,
+      c_void_p, c_int64, c_int, c_void_p]),
     ("moe_expert_ffn_fp8_workspace_bytes", c_size_t,
      [c_int, c_int, c_int, c_int]),
     ("moe_expert_ffn_fp8_fwd", c_int,

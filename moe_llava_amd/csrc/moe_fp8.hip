@@ -514,6 +514,24 @@ static int fp8_args_ok(const char *fn, const void *a, int64_t lda, const void *a
     return 0;
 }
 
+static Fp8GemmParams plain_params(const void *a, int64_t lda, const void *a_scale, int64_t ld_as, const int32_t *gather,
+                                  int gather_shift, const void *w, const void *w_scale, const void *bias,
+                                  const int32_t *group_offsets, int G, int n_experts, int max_rows, int K, int N, int zero_tail,
+                                  void *out, int64_t ldo) {
+    const int nk = (K + QB - 1) / QB, nb = (N + QB - 1) / QB;
+    Fp8GemmParams p{};
+    p.a = (const u8 *)a; p.lda = lda; p.a_scale = (const u8 *)a_scale; p.ld_as = ld_as;
+    p.gather = gather; p.gather_shift = gather_shift;
+    p.w = (const u8 *)w; p.w_expert_stride = (long long)N * K;
+    p.w_scale = (const u8 *)w_scale; p.ws_expert_stride = (long long)nb * nk;
+    p.bias = (const bf16_t *)bias; p.bias_expert_stride = N;
+    p.group_offsets = group_offsets; p.G = G; p.n_experts = n_experts; p.max_rows = max_rows;
+    p.out = out; p.ldo = ldo; p.K = K; p.N_out = N; p.n_gated = N;
+    p.vec_store = aligned16(out) && (ldo & 7) == 0;
+    p.zero_tail = zero_tail != 0 && group_offsets != nullptr;
+    return p;
+}
+
 }  // namespace moe
 
 using namespace moe;
@@ -529,17 +547,42 @@ extern "C" int moe_grouped_gemm_fp8_fwd(const void *a, int64_t lda, const void *
     if (rc) return rc;
     if (ldo < N) return fail(MOE_ERR_SHAPE, "%s: output row stride %lld < N", fn, (long long)ldo);
     if (reinterpret_cast<uintptr_t>(out) & 1) return fail(MOE_ERR_ALIGN, "%s: out must be 2-byte aligned", fn);
-    const int nk = (K + QB - 1) / QB, nb = (N + QB - 1) / QB;
-    Fp8GemmParams p{};
-    p.a = (const u8 *)a; p.lda = lda; p.a_scale = (const u8 *)a_scale; p.ld_as = ld_as;
-    p.gather = gather; p.gather_shift = gather_shift;
-    p.w = (const u8 *)w; p.w_expert_stride = (long long)N * K;
-    p.w_scale = (const u8 *)w_scale; p.ws_expert_stride = (long long)nb * nk;
-    p.bias = (const bf16_t *)bias; p.bias_expert_stride = N;
-    p.group_offsets = group_offsets; p.G = G; p.n_experts = n_experts_local; p.max_rows = max_rows;
-    p.out = out; p.ldo = ldo; p.K = K; p.N_out = N; p.n_gated = N;
-    p.vec_store = aligned16(out) && (ldo & 7) == 0;
-    p.zero_tail = zero_tail != 0;
+    return fp8_gemm(plain_params(a, lda, a_scale, ld_as, gather, gather_shift, w, w_scale, bias, group_offsets, G, n_experts_local,
+                                 max_rows, K, N, zero_tail, out, ldo),
+                    MOE_EPI_PLAIN, dtype, (hipStream_t)stream);
+}
+
+extern "C" size_t moe_grouped_linear_fp8_workspace_bytes(int rows, int K) {
+    if (rows < 0 || K < 1) return 0;
+    const size_t q = ((size_t)rows * K + 255) & ~(size_t)255;
+    return q + (size_t)rows * (((K + QB - 1) / QB + 3) / 4 * 4);
+}
+
+extern "C" int moe_grouped_linear_fp8_fwd(const void *x, int64_t ldx, const void *w, const void *w_scale, const void *bias,
+                                          const int32_t *group_offsets, int G, int n_experts_local, int rows, int K, int N,
+                                          int zero_tail, void *workspace, size_t ws_bytes, void *out, int64_t ldo, int dtype,
+                                          void *stream) {
+    const char *fn = "moe_grouped_linear_fp8_fwd";
+    if (!x || !workspace || !out || (!group_offsets && G != 1)) return fail(MOE_ERR_ARG, "%s: null pointer", fn);
+    if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
+    const long long ld_as = ((K + QB - 1) / QB + 3) / 4 * 4;
+    // the product's own rules first, so that a bad call launches nothing
+    int rc = fp8_args_ok(fn, workspace, K, workspace, ld_as, 0, w, w_scale, bias, G, n_experts_local, rows, K, N);
+    if (rc) return rc;
+    if (ldo < N || (rows > 1 && ldx < K)) return fail(MOE_ERR_SHAPE, "%s: row strides %lld, %lld: need >= K, >= N", fn, (long long)ldx, (long long)ldo);
+    if ((reinterpret_cast<uintptr_t>(x) & 1) || (reinterpret_cast<uintptr_t>(out) & 1)) return fail(MOE_ERR_ALIGN, "%s: x and out must be 2-byte aligned", fn);
+    if (ws_bytes < moe_grouped_linear_fp8_workspace_bytes(rows, K)) return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes too small", fn, ws_bytes);
+    if (rows == 0) return 0;
+    u8 *q = (u8 *)workspace, *qs = q + (((size_t)rows * K + 255) & ~(size_t)255);
+    Fp8GemmParams p = plain_params(q, K, qs, ld_as, nullptr, 0, w, w_scale, bias, group_offsets, G, n_experts_local, rows, K, N,
+                                   zero_tail, out, ldo);
+    // few rows: quantised on load, when wide loads can fetch them
+    if (rows <= FP8_FEW_ROWS && !p.zero_tail && aligned16(x) && (ldx & 7) == 0) {
+        p.x16 = (const bf16_t *)x;
+        p.ldx = ldx;
+    } else if ((rc = moe_quantize_rows_fp8(x, ldx, rows, K, q, K, qs, ld_as, dtype, stream))) {
+        return rc;
+    }
     return fp8_gemm(p, MOE_EPI_PLAIN, dtype, (hipStream_t)stream);
 }
 

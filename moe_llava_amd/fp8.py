@@ -47,6 +47,12 @@ def _empty_rows(S: int, K: int, dev) -> Fp8Rows:
     return Fp8Rows(q, sc[:, :kb] if kb % 4 else sc)
 
 
+#: pointer of the current stream of a device, by index (torch.cuda.current_stream builds a Stream object per call: 1.9 us
+#: of a decode step's host time against 0.1)
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _gpu(t, name: str) -> None:
     if not isinstance(t, Tensor):
         raise TypeError(f"{name}: expected a tensor")
@@ -59,9 +65,12 @@ def _half_rows(x: Tensor, name: str) -> Tensor:
     _gpu(x, name)
     if x.dtype not in ops.HALF_DTYPES:
         raise TypeError(f"{name}: expected bf16 or fp16, got {x.dtype}")
-    if x.dim() < 1:
+    d = x.dim()
+    if d == 2 and x.is_contiguous():
+        return x
+    if d < 1:
         raise ValueError(f"{name}: expected at least one dimension")
-    if x.dim() != 2:
+    if d != 2:
         x = x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(x.shape[:-1].numel(), x.shape[-1])
     if x.shape[1] > 1 and x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         x = x.contiguous()                  # transposed, or rows that overlap (an expanded row)
@@ -101,31 +110,31 @@ def _lead_scale(sc: Tensor) -> int:
 
 
 def _check_weight(w: Tensor, ws: Tensor, name: str, E: int, N: Optional[int], parts: int = 1) -> Tuple[int, int]:
-    """w [E, parts*N, K] with scales [E, parts*ceil(N/128), ceil(K/128)]; returns (N, K)."""
-    for t, n, dt in ((w, name, E4M3), (ws, f"{name}_scale", E8M0)):
-        _gpu(t, n)
-        if t.dtype != dt:
-            raise TypeError(f"{n}: expected {dt}, got {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError(f"{n}: must be contiguous")
-    n, K = w.shape[-2], w.shape[-1]
-    if n % parts or (N is not None and n != parts * N):
-        raise ValueError(f"{name}: {tuple(w.shape)} does not hold {parts} projection(s) of the expected width")
+    """w [E, parts*N, K] (E == 0: [N, K]) with scales [E, parts*ceil(N/128), ceil(K/128)]; returns (N, K)."""
+    _gpu(w, name)
+    _gpu(ws, f"{name}_scale")
+    if w.dtype != E4M3 or ws.dtype != E8M0:
+        raise TypeError(f"{name}: expected {E4M3} with {E8M0} scales, got {w.dtype} with {ws.dtype}")
+    if not (w.is_contiguous() and ws.is_contiguous()):
+        raise ValueError(f"{name} and its scales must be contiguous")
+    sh, sc = w.shape, ws.shape
+    nd = 3 if E else 2
+    if len(sh) != nd or len(sc) != nd:
+        raise ValueError(f"{name}: {tuple(sh)} with scales {tuple(sc)}: need {'[E, N, K]' if E else '[N, K]'}")
+    n, K = sh[-2], sh[-1]
+    if n < parts or n % parts or (N is not None and n != parts * N):
+        raise ValueError(f"{name}: {tuple(sh)} does not hold {parts} projection(s) of the expected width")
     n //= parts
     if K % 16 or not 16 <= K <= MAX_K:
         raise ValueError(f"{name}: K={K} must be a multiple of 16 and at most {MAX_K}")
-    if ws.device != w.device or tuple(ws.shape) != tuple(w.shape[:-2]) + (parts * _blocks(n), _blocks(K)):
-        raise ValueError(f"{name}_scale: {tuple(ws.shape)} on {ws.device} does not match {name} {tuple(w.shape)} on {w.device}")
-    if w.dim() == 3 and w.shape[0] != E:
-        raise ValueError(f"{name}: {w.shape[0]} experts, expected {E}")
+    if sc[-2] != parts * _blocks(n) or sc[-1] != _blocks(K) or (E and (sh[0] != E or sc[0] != E)) or ws.device != w.device:
+        raise ValueError(f"{name}_scale: {tuple(sc)} on {ws.device} does not match {name} {tuple(sh)} on {w.device}")
     if w.data_ptr() % 16:
         raise ValueError(f"{name}: must be 16-byte aligned")
     return n, K
 
 
-def _check_bias(b: Optional[Tensor], name: str, shape, dtype, dev) -> None:
-    if b is None:
-        return
+def _check_bias(b: Tensor, name: str, shape, dtype, dev) -> None:
     if not isinstance(b, Tensor) or b.dtype != dtype or tuple(b.shape) != tuple(shape) or b.device != dev \
             or not b.is_contiguous():
         raise ValueError(f"{name}: need a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
@@ -148,7 +157,7 @@ def quantize_rows(x: Tensor) -> Fp8Rows:
     if S:
         with ops._on(x.device):
             rc = _lib.load().moe_quantize_rows_fp8(x.data_ptr(), _lead(x, K), S, K, out.q.data_ptr(), K, out.scale.data_ptr(),
-                                                   _lead_scale(out.scale), ops._dt(x), ops._stream_ptr(x))
+                                                   _lead_scale(out.scale), ops._dt(x), _stream(x.device.index))
         _lib.check(rc, "moe_quantize_rows_fp8")
     return out
 
@@ -170,7 +179,7 @@ def quantize_weight(w: Tensor, projections: int = 1) -> Tuple[Tensor, Tensor]:
     sc = torch.empty(tuple(w.shape[:-2]) + (projections * _blocks(n), _blocks(k)), dtype=E8M0, device=w.device)
     with ops._on(w.device):
         rc = _lib.load().moe_quantize_blocks_fp8(w.data_ptr(), batch, n, k, q.data_ptr(), sc.data_ptr(), ops._dt(w),
-                                                 ops._stream_ptr(w))
+                                                 _stream(w.device.index))
     _lib.check(rc, "moe_quantize_blocks_fp8")
     return q, sc
 
@@ -188,8 +197,27 @@ def _gemm(a: Fp8Rows, w: Tensor, ws: Tensor, bias: Optional[Tensor], offs: Optio
             a.q.data_ptr(), _lead(a.q, K), a.scale.data_ptr(), _lead_scale(a.scale), None, 0, w.data_ptr(), ws.data_ptr(),
             bias.data_ptr() if bias is not None else None, offs.data_ptr() if offs is not None else None, G, E, S, K, N,
             int(zero_tail), out.data_ptr(), N, ops.DTYPE_F16 if dtype == torch.float16 else ops.DTYPE_BF16,
-            ops._stream_ptr(a.q))
+            _stream(a.q.device.index))
     _lib.check(rc, "moe_grouped_gemm_fp8_fwd")
+    return out
+
+
+def _linear16(x: Tensor, w: Tensor, ws: Tensor, bias: Optional[Tensor], offs: Optional[Tensor], E: int, N: int, K: int) -> Tensor:
+    """16-bit rows x [S, K]: quantised and multiplied in one library call."""
+    S = x.shape[0]
+    dev = x.device
+    out = torch.empty((S, N), dtype=x.dtype, device=dev)
+    if S == 0:
+        return out
+    lib = _lib.load()
+    nws = lib.moe_grouped_linear_fp8_workspace_bytes(S, K)
+    buf = torch.empty((nws,), dtype=torch.uint8, device=dev)
+    with ops._on(dev):
+        rc = lib.moe_grouped_linear_fp8_fwd(
+            x.data_ptr(), _lead(x, K), w.data_ptr(), ws.data_ptr(), bias.data_ptr() if bias is not None else None,
+            offs.data_ptr() if offs is not None else None, offs.numel() - 1 if offs is not None else 1, E, S, K, N,
+            int(offs is not None), buf.data_ptr(), nws, out.data_ptr(), N, ops._dt(x), _stream(dev.index))
+    _lib.check(rc, "moe_grouped_linear_fp8_fwd")
     return out
 
 
@@ -202,7 +230,7 @@ class _LinearFn(torch.autograd.Function):
     def forward(ctx, x: Tensor, w: Tensor, ws: Tensor, bias, offs, E: int, N: int, K: int):
         ctx.save_for_backward(w, ws, offs)
         ctx.meta = (E, N, K, x.shape, x.dtype)
-        return _gemm(quantize_rows(x), w, ws, bias, offs, E, N, K, x.dtype, offs is not None)
+        return _linear16(x, w, ws, bias, offs, E, N, K)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -213,50 +241,51 @@ class _LinearFn(torch.autograd.Function):
         wst = torch.empty((E, _blocks(K), _blocks(N)), dtype=E8M0, device=w.device)
         with ops._on(w.device):
             rc = _lib.load().moe_transpose_blocks_fp8(w.data_ptr(), ws.data_ptr(), E, N, K, wt.data_ptr(), wst.data_ptr(),
-                                                      ops._stream_ptr(w))
+                                                      _stream(w.device.index))
         _lib.check(rc, "moe_transpose_blocks_fp8")
-        dx = _gemm(quantize_rows(dy), wt, wst, None, offs, E, K, N, dtype, offs is not None)
+        dx = _linear16(_half_rows(dy, "dy"), wt, wst, None, offs, E, K, N)
         return dx.reshape(shape), None, None, None, None, None, None, None
 
 
 def _linear(x, w: Tensor, ws: Tensor, bias: Optional[Tensor], offs: Optional[Tensor], dtype) -> Tensor:
-    E = w.shape[0] if offs is not None else 1
-    if w.dim() != (3 if offs is not None else 2):
-        raise ValueError(f"w: {tuple(w.shape)}: need {'[E, N, K]' if offs is not None else '[N, K]'}")
+    grouped = offs is not None
+    _gpu(w, "w")
+    E = (w.shape[0] if w.dim() == 3 else -1) if grouped else 0
     N, K = _check_weight(w, ws, "w", E, None)
+    dev = w.device
+    rows = None
     if isinstance(x, Fp8Rows):
         if dtype is None:
             dtype = bias.dtype if bias is not None else torch.bfloat16
         if dtype not in ops.HALF_DTYPES:
             raise TypeError(f"out_dtype: expected bf16 or fp16, got {dtype}")
         rows = _check_rows(x, "x")
-        if rows.q.shape[1] != K or rows.q.device != w.device:
-            raise ValueError(f"x {tuple(rows.q.shape)} on {rows.q.device} does not match w {tuple(w.shape)} on {w.device}")
+        x2 = rows.q
     else:
+        x2 = _half_rows(x, "x")
         if dtype is not None and dtype != x.dtype:
             raise TypeError("out_dtype is the input's type for 16-bit inputs")
-        rows = None
         dtype = x.dtype
-        x2 = _half_rows(x, "x")
-        if x2.shape[1] != K or x2.device != w.device:
-            raise ValueError(f"x {tuple(x.shape)} on {x2.device} does not match w {tuple(w.shape)} on {w.device}")
-    _check_bias(bias, "bias", (E, N) if offs is not None else (N,), dtype, w.device)
-    if offs is not None:
-        _check_index(offs, "group_offsets", w.device)
-        if not 1 <= offs.numel() - 1 <= 4096:
+    if x2.shape[1] != K or x2.device != dev:
+        raise ValueError(f"x {tuple(x2.shape)} on {x2.device} does not match w {tuple(w.shape)} on {dev}")
+    if bias is not None:
+        _check_bias(bias, "bias", (E, N) if grouped else (N,), dtype, dev)
+    if grouped:
+        _check_index(offs, "group_offsets", dev)
+        if not 2 <= offs.numel() <= 4097:
             raise ValueError("group_offsets needs 2 to 4097 entries")
+    E = E or 1
     if rows is not None:
-        return _gemm(rows, w, ws, bias, offs, E, N, K, dtype, offs is not None)
+        return _gemm(rows, w, ws, bias, offs, E, N, K, dtype, grouped)
+    grad = False
     if torch.is_grad_enabled():
         if bias is not None and bias.requires_grad:
             raise NotImplementedError("fp8 products are for frozen weights: bias.requires_grad is not supported")
-        if x.requires_grad:
-            if N % 16 or N > MAX_K:
-                raise NotImplementedError(f"the input gradient needs N % 16 == 0 and N <= {MAX_K} (N={N})")
-            y = _LinearFn.apply(x2, w, ws, bias, offs, E, N, K)
-            return y.reshape(x.shape[:-1] + (N,))
-    y = _gemm(quantize_rows(x2), w, ws, bias, offs, E, N, K, dtype, offs is not None)
-    return y.reshape(x.shape[:-1] + (N,))
+        grad = x.requires_grad
+        if grad and (N % 16 or N > MAX_K):
+            raise NotImplementedError(f"the input gradient needs N % 16 == 0 and N <= {MAX_K} (N={N})")
+    y = (_LinearFn.apply if grad else _linear16)(x2, w, ws, bias, offs, E, N, K)
+    return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (N,))
 
 
 def linear(x: Union[Tensor, Fp8Rows], w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = None, out_dtype=None) -> Tensor:
@@ -290,8 +319,9 @@ def expert_ffn(act, x: Union[Tensor, Fp8Rows], w1: Tensor, w1_scale: Tensor, w2:
     act = _ACTS.get(act, -1)
     if act < 0:
         raise ValueError("act: 'swiglu' or 'gelu_new'")
-    if w1.dim() != 3 or w2.dim() != 3:
-        raise ValueError("w1 / w2: expected [E, N, K]")
+    _gpu(w2, "w2")
+    if w2.dim() != 3 or w2.shape[0] < 1:
+        raise ValueError(f"w2: {tuple(w2.shape)}: need [E, M, I]")
     E = w2.shape[0]
     M, I = _check_weight(w2, w2_scale, "w2", E, None)
     parts = 2 if act == ops.ACT_SWIGLU else 1
@@ -315,8 +345,10 @@ def expert_ffn(act, x: Union[Tensor, Fp8Rows], w1: Tensor, w1_scale: Tensor, w2:
                                       "fp8.grouped_linear, which is differentiable")
     if src.shape[1] != M or src.device != dev or w2.device != dev:
         raise ValueError(f"x {tuple(src.shape)} on {src.device} does not match w1 {tuple(w1.shape)} on {dev}")
-    _check_bias(b1, "b1", (E, parts * I), dtype, dev)
-    _check_bias(b2, "b2", (E, M), dtype, dev)
+    if b1 is not None:
+        _check_bias(b1, "b1", (E, parts * I), dtype, dev)
+    if b2 is not None:
+        _check_bias(b2, "b2", (E, M), dtype, dev)
     _check_index(group_offsets, "group_offsets", dev)
     G = group_offsets.numel() - 1
     if not 1 <= G <= 4096 or max_rows < 0:
@@ -346,6 +378,6 @@ def expert_ffn(act, x: Union[Tensor, Fp8Rows], w1: Tensor, w1_scale: Tensor, w2:
             b1.data_ptr() if b1 is not None else None, w2.data_ptr(), w2_scale.data_ptr(),
             b2.data_ptr() if b2 is not None else None, group_offsets.data_ptr(), G, E, max_rows, M, I, n_gated,
             ws.data_ptr(), nws, y.data_ptr(), ops.DTYPE_F16 if dtype == torch.float16 else ops.DTYPE_BF16,
-            ops._stream_ptr(src))
+            _stream(dev.index))
     _lib.check(rc, "moe_expert_ffn_fp8_fwd")
     return y

@@ -15,7 +15,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib, ops
-from .fp8 import Fp8Rows, _empty_rows, _gpu, _half_rows, _lead
+from .fp8 import Fp8Rows, _empty_rows, _gpu, _half_rows, _lead, _lead_scale, _stream
 
 MAX_M = 65536
 
@@ -46,6 +46,10 @@ def _check(x: Tensor, residual: Optional[Tensor], weight: Tensor):
     return x2, r2, weight, _weight_code(weight, x2)
 
 
+def _as(t: Tensor, x: Tensor) -> Tensor:
+    return t if x.dim() == 2 else t.reshape(x.shape)
+
+
 def _launch(x: Tensor, r: Optional[Tensor], w: Tensor, code: int, eps: float, want_y: bool, want_q: bool, want_rstd: bool):
     S, M = x.shape
     dev = x.device
@@ -59,8 +63,8 @@ def _launch(x: Tensor, r: Optional[Tensor], w: Tensor, code: int, eps: float, wa
                 x.data_ptr(), _lead(x, M), r.data_ptr() if r is not None else None, _lead(r, M) if r is not None else 0,
                 w.data_ptr(), code, eps, S, M, y.data_ptr() if want_y else None, M, s.data_ptr() if s is not None else None,
                 M, rstd.data_ptr() if want_rstd else None, rows.q.data_ptr() if want_q else None, M,
-                rows.scale.data_ptr() if want_q else None, rows.scale.stride(0) if want_q else 0, ops._dt(x),
-                ops._stream_ptr(x))
+                rows.scale.data_ptr() if want_q else None, _lead_scale(rows.scale) if want_q else 0, ops._dt(x),
+                _stream(dev.index))
         _lib.check(rc, "moe_add_rms_norm_fwd")
     return y, s, rstd, rows
 
@@ -70,11 +74,11 @@ class _AddRmsNormFn(torch.autograd.Function):
     def forward(ctx, x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float):
         x2, r2, w, code = _check(x, residual, weight)
         y, s, rstd, _ = _launch(x2, r2, w, code, eps, True, False, True)
-        out_s = s.reshape(x.shape) if s is not None else None
+        out_s = _as(s, x) if s is not None else None
         ctx.save_for_backward(out_s if out_s is not None else x, weight, rstd)
         ctx.has_res = residual is not None
         ctx.set_materialize_grads(False)
-        return (y.reshape(x.shape), out_s) if s is not None else y.reshape(x.shape)
+        return (_as(y, x), out_s) if s is not None else _as(y, x)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -101,9 +105,9 @@ class _AddRmsNormFn(torch.autograd.Function):
                     d2.data_ptr() if d2 is not None else None, _lead(d2, M) if d2 is not None else 0,
                     e2.data_ptr() if e2 is not None else None, _lead(e2, M) if e2 is not None else 0, s2.data_ptr(),
                     _lead(s2, M), w.data_ptr(), code, rstd.data_ptr(), S, M, dx.data_ptr(), M, dw.data_ptr(), ws.data_ptr(),
-                    nws, ops._dt(s2), ops._stream_ptr(s2))
+                    nws, ops._dt(s2), _stream(s2.device.index))
             _lib.check(rc, "moe_add_rms_norm_bwd")
-        dx = dx.reshape(s.shape)
+        dx = _as(dx, s)
         return dx, dx if ctx.has_res else None, dw, None
 
 
@@ -115,7 +119,7 @@ def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-6)
         return _AddRmsNormFn.apply(x, residual, weight, float(eps))
     x2, r2, w, code = _check(x, residual, weight)
     y, s, _, _ = _launch(x2, r2, w, code, float(eps), True, False, False)
-    return y.reshape(x.shape), s.reshape(x.shape)
+    return _as(y, x), _as(s, x)
 
 
 def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
@@ -136,7 +140,7 @@ def add_rms_norm_fp8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps:
     if x2.shape[1] % 16:
         raise ValueError(f"x: row length {x2.shape[1]} must be a multiple of 16 for 8-bit output")
     y, s, _, rows = _launch(x2, r2, w, code, float(eps), want_y, True, False)
-    return rows, (y.reshape(x.shape) if want_y else None), (s.reshape(x.shape) if s is not None else x)
+    return rows, (_as(y, x) if want_y else None), (_as(s, x) if s is not None else x)
 
 
 class RMSNorm(nn.Module):
