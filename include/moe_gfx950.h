@@ -401,7 +401,7 @@ int moe_grouped_gemm_fp8_fwd(const void *a, int64_t lda, const void *a_scale, in
                              int zero_tail, void *out, int64_t ldo, int dtype, void *stream);
 
 /* moe_grouped_linear_fp8_fwd: moe_grouped_gemm_fp8_fwd on 16-bit rows x [rows, K] (row stride ldx elements, any alignment),
- * quantised as moe_quantize_rows_fp8 would, into the workspace or on load.  Workspace contents mean nothing between calls;
+ * quantised into the workspace by a launch in front.  Workspace contents mean nothing between calls;
  * calls that may overlap need one each. */
 size_t moe_grouped_linear_fp8_workspace_bytes(int rows, int K);
 int moe_grouped_linear_fp8_fwd(const void *x, int64_t ldx, const void *w, const void *w_scale, const void *bias,

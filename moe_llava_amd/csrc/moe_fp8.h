@@ -77,15 +77,11 @@ struct Fp8GemmParams {
     int col_tiles, rs;
     int vec_store;            // 16-bit output: rows and pointer allow 16-byte stores
     int zero_tail;            // 16-bit output: rows of [0, max_rows) that belong to no group are set to 0
-    const bf16_t *x16;        // few-row launches: 16-bit rows (row stride ldx elements) quantised on load; a, a_scale unused
-    long long ldx;
-    float *h32;               // few-row launches of a first product: fp32 activations [rows, N_out], quantised by a launch behind
     int dtype;
 };
 
-// Launches of few rows (moe_fp8_gemv.hip): at most FP8_FEW_ROWS of them in all.
+// Plain products of few rows (moe_fp8_gemv.hip); fp8_gemm in moe_fp8.hip says when it is taken.
 constexpr int FP8_FEW_ROWS = 64;
-int launch_fp8_few(const Fp8GemmParams &p, int epilogue, hipStream_t st);
-int launch_quantize_f32(const float *h, int rows, int I, u8 *q, u8 *scale, long long ld_scale, hipStream_t st);
+int launch_fp8_few(const Fp8GemmParams &p, hipStream_t st);
 
 }  // namespace moe

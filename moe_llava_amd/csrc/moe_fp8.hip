@@ -444,7 +444,7 @@ static bool fp8_tile_ok(int bm, int bn, int kq) {
     return true;
 }
 template <int EPI>
-static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p) {
+static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p, double *estimate = nullptr) {
     const int nk = (p.K + QB - 1) / QB, kq = (nk + 3) / 4 * 4;
     const double parts = p.max_rows < p.G ? p.max_rows : p.G;  // groups that can hold rows: half a tile of each is lost
     const Fp8Tile *best = nullptr;
@@ -460,6 +460,7 @@ static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p) {
         if (fill > us) us = fill;
         if (!best || us < best_t) { best = &t; best_t = us; }
     }
+    if (estimate) *estimate = best_t;
     return *best;
 }
 
@@ -484,9 +485,18 @@ static int launch_fp8_gemm(const Fp8GemmParams &p, hipStream_t st) {
 static int fp8_gemm(Fp8GemmParams p, int epilogue, int dtype, hipStream_t st) {
     p.dtype = dtype;
     if (p.max_rows == 0) return 0;
-    // a few rows stream the weights: no tile of the ring kernel has enough blocks for that (32 x 256 tiles at two active
-    // experts: 88 blocks for 256 CUs).  The few-row kernel has no rows to clear: zero_tail launches stay on the tiles.
-    if (p.max_rows <= FP8_FEW_ROWS && !p.zero_tail && (epilogue == MOE_EPI_PLAIN || p.h32)) return launch_fp8_few(p, epilogue, st);
+    // Few rows stream the weights.  The few-row kernel's time is its start and end and the active weights at the HBM rate,
+    // more with 17 to 32 rows a group (two row fragments per weight fragment), twice with more (the weights twice); the tiles'
+    // is choose_fp8_tile's estimate, or the weights at the rate that their fewer blocks reach.  Measured, us (few / tiles):
+    // K 2048, N 5632: 8.0 / 8.8 at 16 rows, 10.0 / 8.9 at 32, 14.6 / 8.9 at 48; K 5632, N 2048: 8.8 / 17.5, 11.6 / 17.6, 17.3 /
+    // 17.6; K = N = 1024: 3.9 / 7.1, 4.8 / 7.2, 6.3 / 7.4.  It has no rows to clear: zero_tail launches stay on the tiles.
+    if (epilogue == MOE_EPI_PLAIN && p.max_rows <= FP8_FEW_ROWS && !p.zero_tail) {
+        const double act = p.max_rows < p.G ? p.max_rows : p.G, mb = act * p.N_out * p.K * 1e-6, per = p.max_rows / act;
+        const double few = (5.0 + mb / 5.2) * (per > 32 ? 2.0 : per > 16 ? 1.25 : 1.0);
+        double tiles = 0;
+        choose_fp8_tile<EPI_PLAIN>(p, &tiles);
+        if (few < (tiles > mb / 4.5 ? tiles : mb / 4.5)) return launch_fp8_few(p, st);
+    }
 #define FP8_EPI(DT_)                                                                   \
     switch (epilogue) {                                                                \
         case MOE_EPI_SWIGLU: return launch_fp8_gemm<DT_, EPI_SWIGLU>(p, st);           \
@@ -574,15 +584,9 @@ extern "C" int moe_grouped_linear_fp8_fwd(const void *x, int64_t ldx, const void
     if (ws_bytes < moe_grouped_linear_fp8_workspace_bytes(rows, K)) return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes too small", fn, ws_bytes);
     if (rows == 0) return 0;
     u8 *q = (u8 *)workspace, *qs = q + (((size_t)rows * K + 255) & ~(size_t)255);
-    Fp8GemmParams p = plain_params(q, K, qs, ld_as, nullptr, 0, w, w_scale, bias, group_offsets, G, n_experts_local, rows, K, N,
+    const Fp8GemmParams p = plain_params(q, K, qs, ld_as, nullptr, 0, w, w_scale, bias, group_offsets, G, n_experts_local, rows, K, N,
                                    zero_tail, out, ldo);
-    // few rows: quantised on load, when wide loads can fetch them
-    if (rows <= FP8_FEW_ROWS && !p.zero_tail && aligned16(x) && (ldx & 7) == 0) {
-        p.x16 = (const bf16_t *)x;
-        p.ldx = ldx;
-    } else if ((rc = moe_quantize_rows_fp8(x, ldx, rows, K, q, K, qs, ld_as, dtype, stream))) {
-        return rc;
-    }
+    if ((rc = moe_quantize_rows_fp8(x, ldx, rows, K, q, K, qs, ld_as, dtype, stream))) return rc;
     return fp8_gemm(p, MOE_EPI_PLAIN, dtype, (hipStream_t)stream);
 }
 
@@ -590,7 +594,6 @@ namespace {
 inline size_t pad256b(size_t b) { return (b + 255) & ~(size_t)255; }
 struct FfnWs {
     u8 *hq, *hs, *aq, *as;
-    float *h32;
     long long ld_hs, ld_as;
     size_t total;
 };
@@ -603,10 +606,8 @@ FfnWs carve_ffn(void *ws, int src_rows, int max_rows, int M, int I) {
     r.ld_as = ((M + QB - 1) / QB + 3) / 4 * 4;
     r.hq = take((size_t)max_rows * I);
     r.hs = take((size_t)max_rows * r.ld_hs);
-    const bool few = max_rows <= FP8_FEW_ROWS;  // the activation leaves the first product in fp32
     r.aq = take((size_t)src_rows * M);
     r.as = take((size_t)src_rows * r.ld_as);
-    r.h32 = (float *)take(few ? (size_t)max_rows * I * 4 : 0);
     r.total = off;
     return r;
 }
@@ -633,7 +634,6 @@ extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int s
     if (!aligned16(workspace) || !aligned16(y)) return fail(MOE_ERR_ALIGN, "%s: workspace and y must be 16-byte aligned", fn);
     const FfnWs ws = carve_ffn(workspace, x ? src_rows : 0, max_rows, M, I);
     if (ws_bytes < ws.total) return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, ws_bytes, ws.total);
-    const bool few = max_rows <= FP8_FEW_ROWS;
     if (x) {
         if (src_rows > 1 && ldx < M) return fail(MOE_ERR_SHAPE, "%s: row stride %lld < M", fn, (long long)ldx);
         if (reinterpret_cast<uintptr_t>(x) & 1) return fail(MOE_ERR_ALIGN, "%s: x must be 2-byte aligned", fn);
@@ -644,9 +644,7 @@ extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int s
     rc = fp8_args_ok(fn, workspace, I, workspace, ws.ld_hs, 0, w2, w2_scale, b2, G, n_experts_local, max_rows, I, M);
     if (rc) return rc;
     if (max_rows == 0) return 0;
-    // few rows: quantised on load, when wide loads can fetch them
-    const bool on_load = x && few && aligned16(x) && (ldx & 7) == 0;
-    if (x && !on_load && (rc = moe_quantize_rows_fp8(x, ldx, src_rows, M, ws.aq, M, ws.as, ws.ld_as, dtype, stream))) return rc;
+    if (x && (rc = moe_quantize_rows_fp8(x, ldx, src_rows, M, ws.aq, M, ws.as, ws.ld_as, dtype, stream))) return rc;
     const bool gated = act == MOE_ACT_SWIGLU;
     const int mb = (M + QB - 1) / QB, ib = (I + QB - 1) / QB;
     Fp8GemmParams p{};
@@ -659,9 +657,7 @@ extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int s
     p.out = ws.hq; p.ldo = I; p.out_scale = ws.hs; p.ld_os = ws.ld_hs;
     p.K = M; p.N_out = I; p.b_row_offset = I; p.b_blk_offset = ib;
     p.n_gated = (n_gated < 0 || n_gated > I) ? I : n_gated;
-    if (few) { p.x16 = on_load ? (const bf16_t *)x : nullptr; p.ldx = ldx; p.h32 = ws.h32; }
     if ((rc = fp8_gemm(p, gated ? MOE_EPI_SWIGLU : MOE_EPI_GELU_NEW, dtype, (hipStream_t)stream))) return rc;
-    if (few && (rc = launch_quantize_f32(ws.h32, max_rows, I, ws.hq, ws.hs, ws.ld_hs, (hipStream_t)stream))) return rc;
-    return moe_grouped_gemm_fp8_fwd(ws.hq, I, ws.hs, ws.ld_hs, nullptr, 0, w2, w2_scale, b2, group_offsets, G, n_experts_local,
-                                    max_rows, I, M, 0, y, M, dtype, stream);
+    p = plain_params(ws.hq, I, ws.hs, ws.ld_hs, nullptr, 0, w2, w2_scale, b2, group_offsets, G, n_experts_local, max_rows, I, M, 0, y, M);
+    return fp8_gemm(p, MOE_EPI_PLAIN, dtype, (hipStream_t)stream);
 }

@@ -85,6 +85,28 @@ def test_linear(S, K, N, dt):
     assert torch.equal(y, y2)
 
 
+@pytest.mark.parametrize("S", [1, 20, 50, 64])
+@pytest.mark.parametrize("K,N,tile", [(1040, 40, 0), (5632, 96, 0), (41088, 16448, 64)])
+def test_few_rows(S, K, N, tile):
+    """The weight-streaming kernel: one and two row fragments, rows behind 32, short last blocks of K and of the columns, more
+    than 64 blocks of K in one wave (the last shape; its weights repeat, so that 64 columns are compared)."""
+    g = torch.Generator().manual_seed(S + K)
+    x = _rows(g, S, K, torch.bfloat16)
+    n = tile or N
+    q, s = R.weights(g, 1, n, K)
+    q, s = q[0], s[0]
+    gq, gs = q.to(DEV), s.to(DEV)
+    if tile:
+        s[:] = s[:1]                            # 64 rows are half a block: every block of the tall matrix has one scale row
+        gq = gq.view(torch.uint8).repeat(N // tile, 1).view(R.E4M3)
+        gs = s.to(DEV).view(torch.uint8).repeat(R.nb(N), 1).view(R.E8M0)
+    y = fp8.linear(x.to(DEV), gq, gs)
+    ref, tol = R.product(R.deq(x), R.deq_stored(q, s))
+    R.check16(y[:, :n], ref, tol, "few rows")
+    if tile:
+        assert torch.equal(y.view(S, N // tile, tile), y[:, :tile].unsqueeze(1).expand(S, N // tile, tile))
+
+
 @pytest.mark.parametrize("S,K,N", [(1, 64, 16), (37, 208, 144), (300, 512, 272), (70, 1040, 640)])
 def test_linear_input_gradient(S, K, N):
     g = torch.Generator().manual_seed(S + K + N)
