@@ -420,6 +420,19 @@ int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int src_rows, co
                            const int32_t *group_offsets, int G, int n_experts_local, int max_rows, int M, int I,
                            int n_gated, void *workspace, size_t ws_bytes, void *y, int dtype, void *stream);
 
+/* moe_block_top2_fp8_fwd: moe_block_top2_fwd_args on 8-bit experts: gate, routing, moe_expert_ffn_fp8_fwd and combine in one
+ * call.  args as there (w1, b1, w2, b2, h_ws and splitk_ws are not read); q holds the 8-bit experts and the FFN's workspace
+ * (moe_expert_ffn_fp8_workspace_bytes(xq ? 0 : S, max_rows, M, I) bytes, max_rows as in moe_block_top2_fwd).  The gate reads the
+ * 16-bit rows args->x; xq / xq_scale, when given, are the same rows in 8 bits (moe_add_rms_norm_fwd writes both), else x is
+ * quantised in front of the experts. */
+typedef struct moe_fp8_experts {
+    const void *w1; const void *w1_scale; const void *b1;
+    const void *w2; const void *w2_scale; const void *b2;
+    const void *xq; int64_t ld_xq; const void *xq_scale; int64_t ld_xs;
+    void *workspace; size_t ws_bytes;
+} moe_fp8_experts;
+int moe_block_top2_fp8_fwd(const moe_block_top2_args *args, const moe_fp8_experts *q);
+
 #ifdef __cplusplus
 }
 #endif

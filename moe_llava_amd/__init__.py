@@ -5,6 +5,8 @@
 """
 from .layer import MoE  # noqa: F401
 from .sharded_moe import MOELayer, TopKGate, capacity_of  # noqa: F401
+from . import fp8, norm  # noqa: F401
 from .experts import Experts, ExpertSpec, register_expert_adapter  # noqa: F401
 
-__all__ = ["MoE", "MOELayer", "TopKGate", "Experts", "ExpertSpec", "register_expert_adapter", "capacity_of"]
+__all__ = ["MoE", "MOELayer", "TopKGate", "Experts", "ExpertSpec", "register_expert_adapter", "capacity_of",
+           "fp8", "norm"]

@@ -98,6 +98,7 @@ _SIGNATURES = [
     ("moe_grouped_linear_fp8_fwd", c_int,
      [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t,
       c_void_p, c_int64, c_int, c_void_p]),
+    ("moe_block_top2_fp8_fwd", c_int, [c_void_p, c_void_p]),
     ("moe_expert_ffn_fp8_workspace_bytes", c_size_t,
      [c_int, c_int, c_int, c_int]),
     ("moe_expert_ffn_fp8_fwd", c_int,
@@ -120,6 +121,16 @@ class BlockTop2Args(ctypes.Structure):
         ("h_ws", c_void_p), ("y", c_void_p), ("out", c_void_p),
         ("splitk_ws", c_void_p), ("splitk_ws_bytes", c_size_t),
         ("dtype", c_int), ("stream", c_void_p),
+    ]
+
+
+class Fp8Experts(ctypes.Structure):
+    """``moe_fp8_experts`` of include/moe_gfx950.h (field for field)."""
+    _fields_ = [
+        ("w1", c_void_p), ("w1_scale", c_void_p), ("b1", c_void_p),
+        ("w2", c_void_p), ("w2_scale", c_void_p), ("b2", c_void_p),
+        ("xq", c_void_p), ("ld_xq", c_int64), ("xq_scale", c_void_p), ("ld_xs", c_int64),
+        ("workspace", c_void_p), ("ws_bytes", c_size_t),
     ]
 
 

@@ -125,6 +125,9 @@ class Experts(nn.Module):
         self._external: bool = False
         #: SwiGLU channels >= n_gated skip the SiLU (RePaMLP experts); -1 = ordinary experts.  Refreshed per forward.
         self.n_gated: int = -1
+        #: the experts run in 8 bits (``quantize_fp8``); the 16-bit parameters stay as they are
+        self.fp8: bool = False
+        self._fp8 = None                      # (device, parameter versions, tensors, parameter addresses)
         self._register_state_dict_hook(_contiguous_state_dict)
 
     # ---- packed weights ----------------------------------------------------------------------
@@ -259,6 +262,52 @@ class Experts(nn.Module):
                         chk.append((d, name, prm, prm.data_ptr(), prm.shape[0]))
         self.__dict__["_fast"] = (chk, result)
 
+    # ---- 8-bit experts -----------------------------------------------------------------------
+    def quantize_fp8(self, on: bool = True) -> None:
+        """Run the experts in 8 bits (``fp8.expert_ffn``) from the next inference call on, or in 16 bits again.  The 16-bit
+        parameters stay: checkpoints are unchanged, and the 8-bit copy is made again when one of them was replaced or
+        changed in place (a write through ``.data`` is not seen: call this again after one)."""
+        self.fp8 = bool(on)
+        self._fp8 = None
+
+    @staticmethod
+    def _versions(params):
+        try:
+            return [p._version for p in params]
+        except RuntimeError:                  # parameters made in inference mode keep no version
+            return None
+
+    def packed_fp8(self, device: torch.device):
+        """(act, w1, w1_scale, b1|None, w2, w2_scale, b2|None) of the 8-bit experts, quantised from ``packed()``.  When the
+        16-bit weights change, the same tensors are filled again: a captured graph that reads them stays valid."""
+        cur = self._fp8
+        if cur is not None and cur[0] == device and self.packed_unchanged() is not None \
+                and cur[1] == self._versions([c[2] for c in self._fast[0]]):
+            return cur[2]
+        from . import fp8
+        act, w1, b1, w2, b2 = self.packed(device)
+        specs = self._specs()
+        params = self._params(specs)
+        self._remember_fast(specs, (act, w1, b1, w2, b2))
+        versions = self._versions(params)
+        if cur is not None and cur[0] == device and cur[1] == versions and cur[3] == self._ptrs and not self._external:
+            return cur[2]
+        nproj = len(specs[0].fc1)
+        old = cur[2] if cur is not None and cur[0] == device else None
+        if old is not None and (old[0] != act or old[1].shape != w1.shape or old[4].shape != w2.shape
+                                or (old[3] is None) != (b1 is None) or (old[6] is None) != (b2 is None)
+                                or (old[3] is not None and old[3].dtype != b1.dtype)):
+            old = None
+        with torch.no_grad():
+            q1, s1 = fp8.quantize_weight(w1, nproj, out=old[1:3] if old else None)
+            q2, s2 = fp8.quantize_weight(w2, out=old[4:6] if old else None)
+            # biases stay in 16 bits; copies, like the weights, so that a call uses one state of them all
+            c1, c2 = (old[3].copy_(b1) if b1 is not None else None, old[6].copy_(b2) if b2 is not None else None) if old \
+                else (b1.clone() if b1 is not None else None, b2.clone() if b2 is not None else None)
+        out = old if old else (act, q1, s1, c1, q2, s2, c2)
+        self._fp8 = (device, versions, out, self._ptrs)
+        return out
+
     def _views(self, specs, pk):
         """(nn.Linear, weight view, bias view | None) of every projection in the packed buffers ``pk``."""
         I = specs[0].fc1[0].weight.shape[0]
@@ -307,6 +356,8 @@ class Experts(nn.Module):
             raise ValueError(f"Experts.forward expects [ep, {self.num_local_experts}, C, M], got {tuple(inputs.shape)}")
         ep, el, C, M = inputs.shape
         flat = inputs.contiguous().reshape(ep * el * C, M)
+        if self.fp8:
+            raise NotImplementedError("Experts.forward takes 16-bit experts: 8-bit experts run through MoE / MOELayer")
         act, w1, b1, w2, b2 = self.packed(flat.device)
         offs = torch.arange(0, (ep * el + 1) * C, C, dtype=torch.int32, device=flat.device)
         y = ops.expert_ffn(act, flat, None, 0, w1, b1, w2, b2, offs, ep * el * C, n_gated=self.n_gated)

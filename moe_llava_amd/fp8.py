@@ -14,6 +14,7 @@ The reference has no counterpart: its experts run in 16 bits.  As in ``ops``, no
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -162,9 +163,10 @@ def quantize_rows(x: Tensor) -> Fp8Rows:
     return out
 
 
-def quantize_weight(w: Tensor, projections: int = 1) -> Tuple[Tensor, Tensor]:
+def quantize_weight(w: Tensor, projections: int = 1, out=None) -> Tuple[Tensor, Tensor]:
     """16-bit weights [.., N, K] (K % 16 == 0) -> (e4m3 [.., N, K], scales [.., projections * ceil(N'/128), ceil(K/128)]).
-    ``projections`` = 2 for a gated W1 [.., 2I, M]: each half gets blocks of its own (N' = I)."""
+    ``projections`` = 2 for a gated W1 [.., 2I, M]: each half gets blocks of its own (N' = I).
+    ``out``: (weights, scales) of an earlier call of the same shape, filled again."""
     _gpu(w, "w")
     if w.dtype not in ops.HALF_DTYPES:
         raise TypeError(f"w: expected bf16 or fp16, got {w.dtype}")
@@ -175,8 +177,15 @@ def quantize_weight(w: Tensor, projections: int = 1) -> Tuple[Tensor, Tensor]:
         w = w.clone()
     n, k = w.shape[-2] // projections, w.shape[-1]
     batch = w.numel() // (n * k)
-    q = torch.empty(w.shape, dtype=E4M3, device=w.device)
-    sc = torch.empty(tuple(w.shape[:-2]) + (projections * _blocks(n), _blocks(k)), dtype=E8M0, device=w.device)
+    shape_s = tuple(w.shape[:-2]) + (projections * _blocks(n), _blocks(k))
+    if out is None:
+        q = torch.empty(w.shape, dtype=E4M3, device=w.device)
+        sc = torch.empty(shape_s, dtype=E8M0, device=w.device)
+    else:
+        q, sc = out
+        for t, dt, shape in ((q, E4M3, tuple(w.shape)), (sc, E8M0, shape_s)):
+            if t.dtype != dt or tuple(t.shape) != shape or t.device != w.device or not t.is_contiguous():
+                raise ValueError(f"out: need a contiguous {dt} tensor of shape {shape} on {w.device}")
     with ops._on(w.device):
         rc = _lib.load().moe_quantize_blocks_fp8(w.data_ptr(), batch, n, k, q.data_ptr(), sc.data_ptr(), ops._dt(w),
                                                  _stream(w.device.index))
@@ -381,3 +390,86 @@ def expert_ffn(act, x: Union[Tensor, Fp8Rows], w1: Tensor, w1_scale: Tensor, w2:
             _stream(dev.index))
     _lib.check(rc, "moe_expert_ffn_fp8_fwd")
     return y
+
+
+# ------------------------------------------------------------------------------------------------ whole block
+def check_experts(x: Tensor, experts) -> Tuple[int, int, int]:
+    """(M, I, E) of what ``Experts.packed_fp8`` returns, checked against the rows x [S, M]."""
+    act, w1, s1, b1, w2, s2, b2 = experts
+    ops._need(x, "x", ops.HALF_DTYPES, 2)
+    S, M = x.shape
+    E = w2.shape[0]
+    if _check_weight(w2, s2, "w2", E, M)[1] % 16 or S < 1:
+        raise ValueError(f"w2 {tuple(w2.shape)} / x {tuple(x.shape)}: need multiples of 16, and at least one token")
+    I = w2.shape[2]
+    parts = 2 if act == ops.ACT_SWIGLU else 1
+    dev = x.device
+    if _check_weight(w1, s1, "w1", E, I, parts)[1] != M or w1.device != dev or w2.device != dev:
+        raise ValueError(f"w1 {tuple(w1.shape)} / w2 {tuple(w2.shape)} do not match x {tuple(x.shape)} on {dev}")
+    if b1 is not None:
+        _check_bias(b1, "b1", (E, parts * I), x.dtype, dev)
+    if b2 is not None:
+        _check_bias(b2, "b2", (E, M), x.dtype, dev)
+    return M, I, E
+
+
+def row_pointers(rows: Fp8Rows, S: int, M: int, dev):
+    """(q, row stride, scales, their row stride) for a library call on rows [S, M]."""
+    rows = _check_rows(rows, "rows")
+    if tuple(rows.q.shape) != (S, M) or rows.q.device != dev:
+        raise ValueError(f"rows {tuple(rows.q.shape)} do not match x {(S, M)}")
+    return rows.q.data_ptr(), _lead(rows.q, M), rows.scale.data_ptr(), _lead_scale(rows.scale)
+
+
+def block_top2(x: Tensor, wg_weight: Tensor, capacity: int, noise: Optional[Tensor], noise_seed: int, drop_tokens: bool,
+               experts, n_gated: int = -1, noise_seed_dev: Optional[Tensor] = None, rows: Optional[Fp8Rows] = None):
+    """``ops.block_top2`` on 8-bit experts: gate -> top-2 routing -> expert MLPs -> combine in one library call.  ``experts``:
+    what ``Experts.packed_fp8`` returns; ``rows``: x in 8 bits (the gate reads x).  Returns (out, logits, Routing)."""
+    M, I, E = check_experts(x, experts)
+    act, w1, s1, b1, w2, s2, b2 = experts
+    S, dev = x.shape[0], x.device
+    wgd = ops._wg_dt(wg_weight, x)
+    ops._need(wg_weight, "wg.weight", wg_weight.dtype, 2)
+    if tuple(wg_weight.shape) != (E, M) or wg_weight.device != dev:
+        raise ValueError("wg.weight does not match x and the experts")
+    if noise is not None:
+        ops._need(noise, "noise", torch.float32, 2)
+        if tuple(noise.shape) != (S, E) or noise.device != dev:
+            raise ValueError("noise must be [S, E] on x's device")
+    if noise_seed_dev is not None:
+        ops._need(noise_seed_dev, "noise_seed_dev", torch.int64)
+        if noise is not None or noise_seed_dev.numel() != 1 or noise_seed_dev.device != dev:
+            raise ValueError("noise_seed_dev: one int64 on x's device, and no noise tensor with it")
+    if rows is not None:
+        rows = _check_rows(rows, "rows")
+    max_rows = min(2 * S, E * int(capacity)) if drop_tokens else 2 * S
+    lib = _lib.load()
+    wsr = lib.moe_routing_workspace_bytes(S, E)
+    r = ops.Routing.allocate(S, E, 2, max_rows, int(capacity), wsr, dev)
+    logits = torch.empty((S, E), dtype=torch.float32, device=dev)
+    nws = max(lib.moe_expert_ffn_fp8_workspace_bytes(0 if rows is not None else S, max_rows, M, I), 256)
+    ybytes = (max(max_rows, 1) * M * 2 + 255) // 256 * 256
+    buf = torch.empty((ybytes + nws,), dtype=torch.uint8, device=dev)    # y, then the experts' workspace
+    out = torch.empty((S, M), dtype=x.dtype, device=dev)
+    a = _lib.BlockTop2Args()
+    a.x, a.wg, a.wg_dtype, a.logits = x.data_ptr(), wg_weight.data_ptr(), wgd, logits.data_ptr()
+    a.noise = noise.data_ptr() if noise is not None else None
+    a.noise_seed = int(noise_seed) & 0xFFFFFFFFFFFFFFFF
+    a.noise_seed_dev = noise_seed_dev.data_ptr() if noise_seed_dev is not None else None
+    a.S, a.M, a.E, a.I, a.act, a.capacity = S, M, E, I, act, int(capacity)
+    a.drop_tokens, a.n_gated = int(bool(drop_tokens)), n_gated
+    for name in ("expert_idx", "slot", "weight", "exp_counts", "kept_counts", "expert_offsets", "perm", "l_aux"):
+        setattr(a, name, r.ptr(name))
+    a.routing_ws, a.routing_ws_bytes = r.ptr("workspace"), wsr
+    a.y, a.out, a.dtype, a.stream = buf.data_ptr(), out.data_ptr(), ops._dt(x), _stream(dev.index)
+    q = _lib.Fp8Experts()
+    q.w1, q.w1_scale, q.b1 = w1.data_ptr(), s1.data_ptr(), b1.data_ptr() if b1 is not None else None
+    q.w2, q.w2_scale, q.b2 = w2.data_ptr(), s2.data_ptr(), b2.data_ptr() if b2 is not None else None
+    if rows is not None:
+        q.xq, q.ld_xq, q.xq_scale, q.ld_xs = row_pointers(rows, S, M, dev)
+    q.workspace, q.ws_bytes = buf.data_ptr() + ybytes, nws
+    with ops._on(dev):
+        rc = lib.moe_block_top2_fp8_fwd(ctypes.byref(a), ctypes.byref(q))
+    _lib.check(rc, "moe_block_top2_fp8_fwd")
+    r._keep = buf
+    return out, logits, r

@@ -63,6 +63,8 @@ class GraphedMoE:
                     self.out = self._forward()
         finally:
             gate.__dict__.pop("noise_seed_dev", None)
+        # 8-bit experts: the graph reads this copy of them; the reference keeps it alive, __call__ keeps it up to date
+        self._fp8 = layer.experts.packed_fp8(dev) if layer.experts.fp8 else None
         self.routing = layer.last_routing      # static routing arrays of the captured step (overwritten per replay)
 
     def _forward(self):
@@ -75,6 +77,9 @@ class GraphedMoE:
         if x.shape != self.x.shape or x.dtype != self.x.dtype or x.device != self.x.device:
             raise ValueError(f"GraphedMoE: captured for {tuple(self.x.shape)} {self.x.dtype} on {self.x.device}, got "
                              f"{tuple(x.shape)} {x.dtype} on {x.device}")
+        experts = self.layer.experts
+        if (experts.packed_fp8(x.device) if experts.fp8 else None) is not self._fp8:
+            raise ValueError("GraphedMoE: captured on another form of the experts (16-bit, or another 8-bit copy): capture again")
         self.x.copy_(x)
         self.graph.replay()
         return self.out

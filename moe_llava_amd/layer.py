@@ -61,6 +61,32 @@ class MoE(nn.Module):
     def set_ep_group(self, group) -> None:
         self.deepspeed_moe._set_ep_group(group)
 
+    def quantize_experts(self, on: bool = True) -> "MoE":
+        """Run the experts in 8 bits from now on (``fp8``: e4m3 with a power-of-two scale per block of 128), or in 16 bits
+        again with ``on=False``.  Inference on one GPU; gate, routing, combine and the 16-bit parameters stay as they are."""
+        if on and self.ep_size > 1:
+            raise NotImplementedError("8-bit experts run on one GPU (ep_size == 1)")
+        self.deepspeed_moe.experts.quantize_fp8(on)
+        return self
+
+    def forward_normed(self, hidden_states: Tensor, residual: Tensor, norm: nn.Module, used_token: Optional[Tensor] = None):
+        """The step of a pre-norm decoder layer in front of and through the block: ``s = hidden_states + residual``,
+        ``forward(rms_norm(s))``.  Returns ``(output, l_aux, exp_counts, s)``; the layer's output is ``s + output``.  ``norm``:
+        a module with ``weight`` and ``eps`` (or ``variance_epsilon``).  With 8-bit experts the norm's launch writes the rows in
+        8 bits beside the 16-bit rows that the gate reads, otherwise this is ``norm.add_rms_norm`` and ``forward``."""
+        from . import norm as norm_ops
+        eps = getattr(norm, "eps", None)
+        if eps is None:
+            eps = norm.variance_epsilon
+        layer = self.deepspeed_moe
+        if not self.use_residual and layer.takes_fp8_rows(hidden_states, used_token):
+            rows, y, s = norm_ops.add_rms_norm_fp8(hidden_states, residual, norm.weight, eps)
+            out = layer(y, used_token, rows)
+            return out, layer.l_aux, layer.exp_counts, s
+        y, s = norm_ops.add_rms_norm(hidden_states, residual, norm.weight, eps)
+        out, l_aux, exp_counts = self(y, used_token)
+        return out, l_aux, exp_counts, s
+
     def forward(self, hidden_states: Tensor, used_token: Optional[Tensor] = None, *args, **kwargs):
         """Returns ``(output, l_aux, exp_counts)``: output has the input's shape and dtype, ``l_aux`` is a 0-dim
         fp32 tensor, ``exp_counts`` an int64 ``[num_experts]`` tensor (pre-drop counts)."""

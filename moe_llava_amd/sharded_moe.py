@@ -165,17 +165,23 @@ class _DecodePlan:
     fresh tensor every time."""
 
     __slots__ = ("args", "ref", "routing", "logits", "hy", "packed", "S", "M", "cap", "sampling", "fn", "l_aux", "exp_counts",
-                 "dtype", "dev")
+                 "dtype", "dev", "q", "qref")
 
     def __init__(self, layer: "MOELayer", x: Tensor, packed, st: int):
+        """``packed``: ``Experts.packed()`` or, for 8-bit experts, ``Experts.packed_fp8()``."""
         from . import _lib
         gate, experts = layer.gate, layer.experts
-        act, w1, b1, w2, b2 = packed
+        eight = experts.fp8
+        act, w1, b1, w2, b2 = (packed[0], packed[1], packed[3], packed[4], packed[6]) if eight else packed
         wgw = gate.wg.weight
         S, M = x.shape
         E, I = wgw.shape[0], w2.shape[2]
         # the same validation the general path does per call, once
-        ops._check_ffn_weights(act, x, w1, b1, w2, b2)
+        if eight:
+            from . import fp8
+            fp8.check_experts(x, packed)
+        else:
+            ops._check_ffn_weights(act, x, w1, b1, w2, b2)
         ops._need(wgw, "wg.weight", wgw.dtype, 2)
         if wgw.shape[1] != M or wgw.device != x.device or w1.shape[0] != E:
             raise ValueError("wg.weight / expert weights do not match x")
@@ -187,7 +193,12 @@ class _DecodePlan:
         r = ops.Routing.allocate(S, E, 2, max_rows, cap, ws_bytes, x.device)
         rows = max(max_rows, 1)
         self.logits = torch.empty((S, E), dtype=torch.float32, device=x.device)
-        self.hy = torch.empty((rows * (I + M),), dtype=x.dtype, device=x.device)
+        if eight:
+            nws = lib.moe_expert_ffn_fp8_workspace_bytes(S, rows, M, I)
+            yb = (rows * M * 2 + 255) // 256 * 256
+            self.hy = torch.empty((yb + nws,), dtype=torch.uint8, device=x.device)      # y, then the experts' workspace
+        else:
+            self.hy = torch.empty((rows * (I + M),), dtype=x.dtype, device=x.device)
         a = _lib.BlockTop2Args()
         a.wg, a.wg_dtype, a.logits = wgw.data_ptr(), ops._wg_dt(wgw, x), self.logits.data_ptr()
         a.noise, a.noise_seed, a.noise_seed_dev = None, 0, None
@@ -199,18 +210,27 @@ class _DecodePlan:
         a.w1, a.b1 = w1.data_ptr(), (b1.data_ptr() if b1 is not None else None)
         a.w2, a.b2 = w2.data_ptr(), (b2.data_ptr() if b2 is not None else None)
         hp = self.hy.data_ptr()
-        a.h_ws, a.y = hp, hp + rows * I * 2
+        if eight:
+            a.h_ws, a.y = None, hp
+            q = self.q = _lib.Fp8Experts()
+            q.w1, q.w1_scale, q.b1 = w1.data_ptr(), packed[2].data_ptr(), a.b1
+            q.w2, q.w2_scale, q.b2 = w2.data_ptr(), packed[5].data_ptr(), a.b2
+            q.workspace, q.ws_bytes = hp + yb, nws
+            self.qref = ctypes.byref(q)
+        else:
+            a.h_ws, a.y = hp, hp + rows * I * 2
+            self.q = None
         a.splitk_ws, a.splitk_ws_bytes = None, 0         # decode-size launches take the GEMV-style kernel: nothing to split
         a.dtype, a.stream = ops._dt(x), st
         self.args, self.ref = a, ctypes.byref(a)
         self.routing, self.packed, self.S, self.M, self.cap = r, packed, S, M, cap
         self.sampling = bool(gate.top2_2nd_expert_sampling)
-        self.fn = lib.moe_block_top2_fwd_args
+        self.fn = lib.moe_block_top2_fp8_fwd if eight else lib.moe_block_top2_fwd_args
         self.l_aux, self.exp_counts = r.l_aux, r.exp_counts      # views, created once
         self.dtype, self.dev = x.dtype, x.device
         r._keep = (self.hy, wgw)
 
-    def run(self, gate: "TopKGate", x: Tensor) -> Tensor:
+    def run(self, gate: "TopKGate", x: Tensor, rows8=None) -> Tensor:
         a = self.args
         seed_dev = gate.__dict__.get("noise_seed_dev")            # graph.GraphedMoE: the seed lives on the device
         noise = gate.noise_override
@@ -227,10 +247,19 @@ class _DecodePlan:
             a.noise, a.noise_seed, a.noise_seed_dev = None, _fresh_seed(), None
         out = torch.empty((self.S, self.M), dtype=self.dtype, device=self.dev)
         a.x, a.out = x.data_ptr(), out.data_ptr()
-        rc = self.fn(self.ref)
+        if self.q is not None:
+            q = self.q
+            if rows8 is not None:
+                from . import fp8
+                q.xq, q.ld_xq, q.xq_scale, q.ld_xs = fp8.row_pointers(rows8, self.S, self.M, self.dev)
+            else:
+                q.xq, q.ld_xq, q.xq_scale, q.ld_xs = None, 0, None, 0
+            rc = self.fn(self.ref, self.qref)
+        else:
+            rc = self.fn(self.ref)
         if rc:
             from . import _lib
-            _lib.check(rc, "moe_block_top2_fwd_args")
+            _lib.check(rc, "moe_block_top2_fp8_fwd" if self.q is not None else "moe_block_top2_fwd_args")
         return out
 
 
@@ -322,6 +351,7 @@ class MOELayer(nn.Module):
     def forward(self, *inp) -> Tensor:
         x_in = inp[0]
         used_token = inp[1] if len(inp) > 1 else None
+        rows8 = inp[2] if len(inp) > 2 else None             # x_in's rows in 8 bits (MoE.forward_normed)
         if x_in.dtype not in ops.HALF_DTYPES:
             # the reference trains and serves with --bf16 (scripts/v1/*/finetune_moe.sh) and builds the model in fp16 in
             # its inference loader (moellava/model/builder.py:70,475; serve/cli.py:67-69): both run, nothing else does
@@ -332,6 +362,9 @@ class MOELayer(nn.Module):
         if torch.is_grad_enabled():
             params = self.experts.param_list()
             if x_in.requires_grad or wg.requires_grad or any(p.requires_grad for p in params):
+                if self.experts.fp8:
+                    raise NotImplementedError("8-bit experts are for inference: wrap the call in torch.no_grad(), or go back "
+                                              "with quantize_experts(False)")
                 if x_in.dtype != torch.bfloat16:
                     raise NotImplementedError("training runs in bf16 (as the reference's scripts do, --bf16 True); the fp16 "
                                               "path is forward only: wrap inference in torch.no_grad()")
@@ -340,7 +373,7 @@ class MOELayer(nn.Module):
                 out, self.l_aux = _MoEBlockFn.apply(self, used_token, x_in, wg, *params)
                 return out
         with ops.stream_scope(x_in):
-            out, l_aux, _ = self._run(x_in, used_token, save=False)
+            out, l_aux, _ = self._run(x_in, used_token, save=False, rows8=rows8)
         self.__dict__["l_aux"] = l_aux
         return out
 
@@ -357,7 +390,20 @@ class MOELayer(nn.Module):
         d["l_aux"] = torch.full((), float("nan"), dtype=torch.float32, device=x_in.device)
         return x_in * 0 if (torch.is_grad_enabled() and x_in.requires_grad) else torch.empty_like(x_in)
 
-    def _run(self, x_in: Tensor, used_token, save: bool):
+    def takes_fp8_rows(self, x: Tensor, used_token) -> bool:
+        """Whether a call with these arguments runs the one-call inference path on 8-bit experts, which can be handed rows
+        that are in 8 bits already."""
+        return bool(self.experts.fp8 and not torch.is_grad_enabled() and x.is_cuda and x.numel() and x.shape[-1] % 16 == 0
+                    and self._one_call(used_token if self.gate.k != 2 else None))
+
+    def _one_call(self, used_token) -> bool:
+        """One GPU, top-2, nothing between the steps that anybody watches: the whole block in one library call."""
+        gate = self.gate
+        return (self.ep_size == 1 and not (self.force_exchange and self.ep_group is not None) and self.timer is None
+                and used_token is None and gate.k == 2 and not module_has_hooks(gate.wg)
+                and not (gate.noisy_gate_policy == "Jitter" and gate.training))
+
+    def _run(self, x_in: Tensor, used_token, save: bool, rows8=None):
         """gate -> routing -> grouped expert FFN (through the all-to-all when ep_size > 1) -> combine.
         ``save``: keep what the backward needs and return it as the third value."""
         M = x_in.shape[-1]
@@ -370,9 +416,11 @@ class MOELayer(nn.Module):
         if gate.k == 2:
             used_token = None              # ignored by upstream top2gating
         local = self.ep_size == 1 and not (self.force_exchange and self.ep_group is not None)
-        if (local and not save and t is None and used_token is None and gate.k == 2 and not module_has_hooks(gate.wg)
-                and not (gate.noisy_gate_policy == "Jitter" and gate.training)):
+        if not save and self._one_call(used_token):
             # inference on one GPU: the whole block in ONE library call (a decode step is host-bound otherwise)
+            if self.experts.fp8:
+                return self._decode_step(x_in, x, S, rows8) if S <= DECODE_MAX_TOKENS and x.is_cuda \
+                    else self._run_fp8(x_in, x, rows8)
             if S <= DECODE_MAX_TOKENS and x.is_cuda:
                 res = self._decode_step(x_in, x, S)
                 if res is not None:
@@ -401,9 +449,20 @@ class MOELayer(nn.Module):
             t.mark("gate_end")
         d = self.__dict__                  # plain attributes: nn.Module.__setattr__ is slow on this path
         d["exp_counts"], d["last_routing"] = r.exp_counts, r
+        shift = r.top_k - 1                      # perm holds token * top_k + choice
+        if self.experts.fp8:
+            if not local:
+                raise NotImplementedError("8-bit experts run on one GPU (ep_size == 1)")
+            from . import fp8
+            act, w1, s1, b1, w2, s2, b2 = self.experts.packed_fp8(x.device)
+            y = fp8.expert_ffn(act, x, w1, s1, w2, s2, r.expert_offsets, r.max_rows, r.perm, shift, b1, b2,
+                               self.experts.n_gated) if r.max_rows else torch.empty((1, M), dtype=x.dtype, device=x.device)
+            out = ops.combine(y, r, S, M)
+            if t is not None:
+                t.mark("combine_end")
+            return out.reshape(x_in.shape), r.l_aux, None
         act, w1, b1, w2, b2 = self.experts.packed(x.device)
         ng = self.experts.n_gated
-        shift = r.top_k - 1                      # perm holds token * top_k + choice
         saved = None
         if local:
             if save:
@@ -421,12 +480,31 @@ class MOELayer(nn.Module):
                          w2=w2, ng=ng, has_b1=b1 is not None, has_b2=b2 is not None)
         return out.reshape(x_in.shape), r.l_aux, saved
 
-    def _decode_step(self, x_in: Tensor, x: Tensor, S: int):
+    def _run_fp8(self, x_in: Tensor, x: Tensor, rows8):
+        """The one-call path on 8-bit experts (every size; ``rows8``: x in 8 bits)."""
+        from . import fp8
+        gate, experts = self.gate, self.experts
+        packed = experts.packed_fp8(x.device)
+        wgw = gate.wg.weight
+        seed_dev = gate.__dict__.get("noise_seed_dev")        # set by graph.GraphedMoE: seed lives on the device
+        if seed_dev is None or not gate.top2_2nd_expert_sampling or gate.noise_override is not None:
+            seed_dev = None
+            cap, noise, seed = gate._top2_args(x.shape[0], wgw.shape[0])
+        else:
+            cf = gate.capacity_factor if gate.training else gate.eval_capacity_factor
+            cap, noise, seed = capacity_of(x.shape[0], wgw.shape[0], cf * 2, gate.min_capacity), None, 0
+        out, lg, r = fp8.block_top2(x, wgw, cap, noise, seed, gate.drop_tokens, packed, experts.n_gated, seed_dev, rows8)
+        gate.__dict__["last_logits"] = lg
+        d = self.__dict__
+        d["exp_counts"], d["last_routing"] = r.exp_counts, r
+        return out.reshape(x_in.shape), r.l_aux, None
+
+    def _decode_step(self, x_in: Tensor, x: Tensor, S: int, rows8=None):
         """Decode-size forward through a cached ``_DecodePlan`` (see there for what is reused between calls)."""
         gate, experts = self.gate, self.experts
         d = self.__dict__
         st = ops._stream_ptr(x)
-        packed = experts.packed_unchanged()
+        packed = experts.packed_fp8(x.device) if experts.fp8 else experts.packed_unchanged()
         if packed is None:
             packed = experts.packed(x.device)
             experts._remember_fast(experts._specs(), packed)
@@ -437,14 +515,14 @@ class MOELayer(nn.Module):
         if plans is None:
             plans = d["_decode_plans"] = {}
         wgw = gate.wg.weight
-        key = (S, x.dtype, x.device.index, st, gate.training, wgw.data_ptr(), wgw.dtype, gate.capacity_factor,
+        key = (experts.fp8, S, x.dtype, x.device.index, st, gate.training, wgw.data_ptr(), wgw.dtype, gate.capacity_factor,
                gate.eval_capacity_factor, gate.min_capacity, gate.drop_tokens, gate.top2_2nd_expert_sampling)
         plan = plans.get(key)
         if plan is None or plan.packed is not packed:
             if len(plans) >= 32:
                 plans.clear()
             plan = plans[key] = _DecodePlan(self, x, packed, st)
-        out = plan.run(gate, x)
+        out = plan.run(gate, x, rows8)
         gate.__dict__["last_logits"] = plan.logits
         d["exp_counts"], d["last_routing"] = plan.exp_counts, plan.routing
         return out.reshape(x_in.shape), plan.l_aux, None
