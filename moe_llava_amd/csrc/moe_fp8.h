@@ -78,6 +78,8 @@ struct Fp8GemmParams {
     int vec_store;            // 16-bit output: rows and pointer allow 16-byte stores
     int zero_tail;            // 16-bit output: rows of [0, max_rows) that belong to no group are set to 0
     int dtype;
+    float *splitk_ws;         // K pieces of the 256 x 256 tiles of a last round (Fp8Sched); NULL: tiles stay whole
+    int split_max;            // most pieces of a tile
 };
 
 // Plain products of few rows (moe_fp8_gemv.hip); fp8_gemm in moe_fp8.hip says when it is taken.

@@ -65,74 +65,123 @@ struct FTile {
     static constexpr int WNT = BNW / 4;                       // weight rows per wave
 };
 
+// The work list of a launch, derived by every block from the device-side group sizes (scalar work).  The eight XCDs (block
+// id mod 8) each take one contiguous eighth of the real tiles, in super-rows of rs row tiles: an XCD works on rs x (32 / rs)
+// tiles at a time, which share their panels in its L2.
+// With a workspace, the Rm < 32 tiles of an XCD's last, partial round are cut along K into s = min(32 / Rm, split_max) pieces
+// that fill the round; a launch behind adds a tile's pieces in K order: no atomics, the same bits from call to call.  A cut
+// tile differs from a whole one only through the order of the fp32 additions.
+constexpr int FP8_XCD_CUS = 32;
+template <int BM>
+struct Fp8Sched {
+    int RT;
+    long long T;
+    __device__ __forceinline__ explicit Fp8Sched(const Fp8GemmParams &p) {
+        RT = 0;
+        if (p.group_offsets) {
+            for (int g = 0; g < p.G; ++g) RT += (p.group_offsets[g + 1] - p.group_offsets[g] + BM - 1) / BM;
+        } else {
+            RT = (p.max_rows + BM - 1) / BM;
+        }
+        T = (long long)RT * p.col_tiles;
+    }
+    __device__ __forceinline__ int tiles(int x) const { return (int)((T >> 3) + (x < (int)(T & 7) ? 1 : 0)); }
+    __device__ __forceinline__ long long start(int x) const {
+        const long long q = T >> 3, r = T & 7;
+        return x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q;
+    }
+    // tiles of XCD x that run whole, and how many pieces each of the others is cut into
+    __device__ __forceinline__ void cut(const Fp8GemmParams &p, int x, int &full, int &rm, int &s) const {
+        const int n = tiles(x);
+        full = n / FP8_XCD_CUS * FP8_XCD_CUS;
+        rm = n - full;
+        s = rm > 0 ? FP8_XCD_CUS / rm : 1;
+        if (s > p.split_max) s = p.split_max;
+        if (!p.splitk_ws || s < 2) { full = n; rm = 0; s = 1; }
+    }
+    __device__ __forceinline__ int whole(const Fp8GemmParams &p, int x) const { int f, r, s; cut(p, x, f, r, s); return f; }
+    __device__ __forceinline__ int items(const Fp8GemmParams &p, int x) const { int f, r, s; cut(p, x, f, r, s); return f + r * s; }
+    __device__ __forceinline__ int most_items(const Fp8GemmParams &p) const {  // of any XCD
+        return (int)(T >> 3) + ((T & 7) ? 1 : 0) + (p.splitk_ws ? FP8_XCD_CUS : 0);
+    }
+    __device__ __forceinline__ bool item(const Fp8GemmParams &p, int x, int i, long long &t, int &piece, int &pieces) const {
+        int full, rm, s;
+        cut(p, x, full, rm, s);
+        piece = 0;
+        pieces = 1;
+        if (i < full) { t = start(x) + i; return true; }
+        const int j = i - full;
+        if (j >= rm * s) return false;
+        t = start(x) + full + j % rm;
+        piece = j / rm;
+        pieces = s;
+        return true;
+    }
+    __device__ __forceinline__ void tile(const Fp8GemmParams &p, long long t, int &ct, int &row_begin, int &row_end, int &expert) const {
+        const long long per = (long long)p.rs * p.col_tiles;
+        const int sr = (int)(t / per), rem = (int)(t - sr * per);
+        const int rin = min(p.rs, RT - sr * p.rs);
+        ct = rem / rin;
+        const int rt = sr * p.rs + (rem - ct * rin);
+        row_begin = rt * BM;
+        row_end = p.max_rows;
+        expert = 0;
+        if (!p.group_offsets) return;
+        int tile0 = 0;
+        for (int g = 0; g < p.G; ++g) {
+            const int b = p.group_offsets[g], e = p.group_offsets[g + 1];
+            const int nt = (e - b + BM - 1) / BM;
+            if (rt < tile0 + nt) {
+                row_begin = b + (rt - tile0) * BM;
+                row_end = e;
+                expert = g % p.n_experts;
+                return;
+            }
+            tile0 += nt;
+        }
+    }
+};
+
 template <int DT, int EPI, int BM, int BNW>
 __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmParams p) {
     using T = FTile<EPI, BM, BNW>;
     typedef Elt<DT> E;
     constexpr int NS = T::NS, NF = T::NF, WNT = T::WNT, NC = T::NC, ROWB = T::ROWB;
+    constexpr bool SPLITS = EPI == EPI_PLAIN && BM == 256 && BNW == 256;  // the tile whose last round is cut along K
     __shared__ __attribute__((aligned(16))) char lds[T::LDS_BYTES];
 
-    // ---- the tile of this block.  The eight XCDs (block id mod 8) each take one contiguous eighth of the real tile list,
-    //      cut on the device from the group sizes; surplus blocks of the worst-case grid exit. ----
-    int RT = 0;
-    if (p.group_offsets) {
-        for (int g = 0; g < p.G; ++g) RT += (p.group_offsets[g + 1] - p.group_offsets[g] + BM - 1) / BM;
-    } else {
-        RT = (p.max_rows + BM - 1) / BM;
-    }
-    const int CT = p.col_tiles;
-    const long long Tn = (long long)RT * CT;
-    int ct = 0, row_begin = 0, row_end = 0, expert = 0;
+    // ---- the work item of this block: a tile, or a piece of a tile's K range (Fp8Sched) ----
+    const int nk = (p.K + QB - 1) / QB;
+    const Fp8Sched<BM> sch(p);
+    int ct = 0, row_begin = 0, row_end = 0, expert = 0, k_lo = 0, k_hi = nk, slot = -1;
     {
-        const int x = blockIdx.x & 7;
-        const long long q8 = Tn >> 3, r8 = Tn & 7;
-        const long long n = q8 + (x < r8 ? 1 : 0), start = x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8;
-        const long long i = blockIdx.x >> 3;
-        if (i >= n) {
-            // surplus block of the worst-case grid.  With zero_tail the grid has at least one more than the tiles on every
+        const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
+        long long t;
+        int piece, pieces;
+        if (!sch.item(p, x, i, t, piece, pieces)) {
+            // surplus block of the worst-case grid.  With zero_tail the grid has at least one more than the items on every
             // XCD: those blocks clear the rows that belong to no group.
-            if (!T::QOUT && p.zero_tail && p.group_offsets) {
-                const long long per_xcd = (long long)(gridDim.x >> 3) - (q8 + (r8 ? 1 : 0));  // surplus blocks of an XCD, at least
-                const long long sid = (i - n) * 8 + x;
+            if (!T::QOUT && p.zero_tail) {
+                const int per_xcd = (int)(gridDim.x >> 3) - sch.most_items(p), k = i - sch.items(p, x);  // surplus of an XCD, at least
                 const int lo = p.group_offsets[0], hi = p.group_offsets[p.G];
-                if (i - n < per_xcd)
-                    for (long long r = sid; r < p.max_rows; r += per_xcd * 8)
+                if (k < per_xcd)
+                    for (long long r = (long long)k * 8 + x; r < p.max_rows; r += per_xcd * 8)
                         if (r < lo || r >= hi)
                             for (int c = threadIdx.x; c < p.N_out; c += FTHREADS) ((bf16_t *)p.out)[r * p.ldo + c] = 0;
             }
             return;
         }
-        const long long t = start + i;
-        // super-rows of rs row tiles: an XCD works on rs x (32 / rs) tiles at a time, which share their panels in its L2
-        const long long per = (long long)p.rs * CT;
-        const int sr = (int)(t / per);
-        const int rem = (int)(t - sr * per);
-        const int rin = min(p.rs, RT - sr * p.rs);
-        ct = rem / rin;
-        const int rt = sr * p.rs + (rem - ct * rin);
-        if (p.group_offsets) {
-            int tile0 = 0;
-            for (int g = 0; g < p.G; ++g) {
-                const int b = p.group_offsets[g], e = p.group_offsets[g + 1];
-                const int nt = (e - b + BM - 1) / BM;
-                if (rt < tile0 + nt) {
-                    row_begin = b + (rt - tile0) * BM;
-                    row_end = e;
-                    expert = g % p.n_experts;
-                    break;
-                }
-                tile0 += nt;
-            }
-        } else {
-            row_begin = rt * BM;
-            row_end = p.max_rows;
+        sch.tile(p, t, ct, row_begin, row_end, expert);
+        if (SPLITS && pieces > 1) {
+            k_lo = piece * nk / pieces;
+            k_hi = (piece + 1) * nk / pieces;
+            slot = x * FP8_XCD_CUS + (i - sch.whole(p, x));
         }
     }
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave & 3, lwave = wave & 3;
-    const int nk = (p.K + QB - 1) / QB;
     const int tail = p.K - (nk - 1) * QB;  // columns of the last slice (a multiple of 16)
     auto xsw = [](int row) { return (row >> 1) & 7; };
     auto src_row = [&](int prow) -> long long {
@@ -224,12 +273,12 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
         if (LOADS) {
 #pragma unroll
             for (int s = 0; s < NS - 1; ++s)
-                if (s < nk) stage(s, s);
+                if (k_lo + s < k_hi) stage(s, k_lo + s);
         } else {
             load_scales();
         }
-        for (int kt = 0; kt < nk; ++kt) {
-            const int ahead = nk - 1 - kt;
+        for (int kt = k_lo; kt < k_hi; ++kt) {
+            const int ahead = k_hi - 1 - kt, at = kt - k_lo;
             static_assert((NS - 2) * PP < 64, "vmcnt field");
             switch (ahead < NS - 2 ? ahead : NS - 2) {
                 case 0: fwait_vm_barrier<0>(); break;
@@ -240,8 +289,8 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
                 case 5: fwait_vm_barrier<(NS > 6 ? 5 : 0) * PP>(); break;
                 default: fwait_vm_barrier<(NS > 7 ? 6 : 0) * PP>(); break;
             }
-            if (LOADS && kt + NS - 1 < nk) stage((kt + NS - 1) % NS, kt + NS - 1);
-            const char *lb = lds + (kt % NS) * T::SLOT;
+            if (LOADS && kt + NS - 1 < k_hi) stage((at + NS - 1) % NS, kt + NS - 1);
+            const char *lb = lds + (at % NS) * T::SLOT;
             const char *xs = lds + T::XS + ((kt >> 2) * BM + row_off + fr) * 4 + (kt & 3);
             constexpr int PD = 2;  // X fragments read ahead
             v8i_t wf[NF], xf[MFW];
@@ -273,6 +322,21 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
                 __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_setprio(0);
+        }
+        if (SPLITS && slot >= 0) {
+            // a piece: the accumulators as they are, 1 KiB per fragment in (lane, register) order; fp8_fixup_kernel adds the
+            // pieces (buffer stores: one register of address, a scalar offset per fragment)
+            float *ws = p.splitk_ws + (size_t)slot * (BM * BNW);
+            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(ws, 0, BM * BNW * 4, 0x00020000);
+            const int sbase = __builtin_amdgcn_readfirstlane(((row_off / 16) * (BNW / 16) + wn * NF) * 1024);
+            typedef unsigned u32x4v_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int nf = 0; nf < NF; ++nf)
+#pragma unroll
+                for (int mf = 0; mf < MFW; ++mf)
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4v_t, acc[nf][mf]), rsrc, lane * 16,
+                                                           sbase + (mf * (BNW / 16) + nf) * 1024, 0);
+            return;
         }
         __syncthreads();  // every wave is done reading the ring
 
@@ -375,6 +439,7 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
         tile_body(FInt<TF - AMF>{}, FInt<0>{}, AMF * 16);
     }
 
+    if (SPLITS && slot >= 0) return;
     // ---- image -> global, 16 bytes a lane; 2 bytes a lane (consecutive lanes, consecutive columns) where the output's rows
     //      do not allow that (8 scattered 2-byte stores a lane took 13 us of a 29.5-us launch, 333 rows, K 1008, N 1003) ----
     typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
@@ -414,16 +479,66 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
     }
 }
 
+// Adds the K pieces of every cut 256 x 256 tile in K order, then bias and the rounding of the plain epilogue.  The waves of a
+// fixed grid take (XCD, tile, fragment) items; a fragment's pieces are read as they were stored, 1 KiB at a time.
+// HBM-bound: pieces * 256 KiB read (at most 64 MiB); 4 us where the device finds nothing to add.
+constexpr int FP8_FIX_BLOCKS = 256, FP8_FIX_THREADS = 1024;
+template <int DT>
+__global__ __launch_bounds__(FP8_FIX_THREADS) void fp8_fixup_kernel(const Fp8GemmParams p) {
+    typedef Elt<DT> E;
+    constexpr int BM = 256, FR = 16;  // fragments per row and column of a tile
+    const Fp8Sched<BM> sch(p);
+    const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
+    const int w0 = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (FP8_FIX_THREADS / 64) + (threadIdx.x >> 6)));
+    constexpr int NW = FP8_FIX_BLOCKS * (FP8_FIX_THREADS / 64);
+    int base = 0;
+    for (int x = 0; x < 8; ++x) {
+        int full, rm, s;
+        sch.cut(p, x, full, rm, s);
+        const int n = rm * FR * FR;
+        // items are dealt over all waves across the XCDs: the first item of XCD x goes to wave base % NW
+        for (int it = (w0 - base % NW + NW) % NW; it < n; it += NW) {
+            const int r = it / (FR * FR), f = it % (FR * FR);
+            int ct, row_begin, row_end, expert;
+            sch.tile(p, sch.start(x) + full + r, ct, row_begin, row_end, expert);
+            const int row = row_begin + (f / FR) * 16 + fr, c0 = ct * 256 + (f % FR) * 16 + fq * 4;
+            f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+            const float *ws = p.splitk_ws + (size_t)(x * FP8_XCD_CUS + r) * (BM * 256) + f * 256 + lane * 4;
+#pragma unroll 4
+            for (int k = 0; k < s; ++k) a += *reinterpret_cast<const f32x4_t *>(ws + (size_t)k * rm * (BM * 256));
+            if (row >= row_end) continue;
+            const bf16_t *bias = p.bias ? p.bias + (long long)expert * p.bias_expert_stride : nullptr;
+            bf16_t *dst = (bf16_t *)p.out + (long long)row * p.ldo + c0;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = a[j] + (bias && c0 + j < p.N_out ? E::to_f(bias[c0 + j]) : 0.f);
+            if (p.vec_store && c0 + 4 <= p.N_out) {
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c0 + j < p.N_out) dst[j] = E::from_f(v[j]);
+            }
+        }
+        base += n;
+    }
+}
+
 template <int DT, int EPI, int BM, int BNW>
 static int launch_fp8_tile(Fp8GemmParams p, hipStream_t st) {
     using T = FTile<EPI, BM, BNW>;
     p.col_tiles = (p.N_out + T::NC - 1) / T::NC;
     p.rs = p.col_tiles <= 8 ? 3 : 4;
     const long long rt = p.group_offsets ? (long long)p.max_rows / BM + p.G : ((long long)p.max_rows + BM - 1) / BM;
-    const long long grid = (rt * p.col_tiles + 7) / 8 * 8 + (p.zero_tail ? 8 : 0);
+    constexpr bool SPLITS = EPI == EPI_PLAIN && BM == 256 && BNW == 256;
+    if (!SPLITS || p.split_max < 2) p.splitk_ws = nullptr;
+    const long long grid = (rt * p.col_tiles + 7) / 8 * 8 + (p.zero_tail ? 8 : 0) + (p.splitk_ws ? 8 * FP8_XCD_CUS : 0);
     if (grid > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "fp8 product: too many tiles (%lld)", grid);
     hipLaunchKernelGGL((fp8_gemm_kernel<DT, EPI, BM, BNW>), dim3((unsigned)grid), dim3(FTHREADS), 0, st, p);
-    return check_launch("fp8_gemm_kernel");
+    int rc = check_launch("fp8_gemm_kernel");
+    if (rc || !p.splitk_ws) return rc;
+    hipLaunchKernelGGL((fp8_fixup_kernel<DT>), dim3(FP8_FIX_BLOCKS), dim3(FP8_FIX_THREADS), 0, st, p);
+    return check_launch("fp8_fixup_kernel");
 }
 
 // Tile choice.  One block runs on a CU at a time, so a launch takes ceil(tiles / 256) rounds of (slices * step + fixed);
@@ -432,6 +547,9 @@ static int launch_fp8_tile(Fp8GemmParams p, hipStream_t st) {
 // per slice with its fills in flight, and prologue + epilogue.  The smallest estimate is within 5 % of the best of
 // twelve tiles on 36 of 40 swept shapes (100 ... 11264 rows, K 1024 ... 10240, N 1024 ... 5632, 1 to 8 groups) and 21 % off
 // at worst; the 256 x 256 tile alone is up to 3.2 x off there (1408 rows, K 5632, N 2048, 4 groups: 57.9 us against 30.9).
+// With a workspace, the 256 x 256 tile's last round may be cut along K (Fp8Sched): its estimate is then the whole rounds, a
+// piece of the tail, and the pieces written and read back (0.11 us each at 4.7 TB/s, 5 us for the launch).  6854 rows, K
+// 10240, N 2560 (290 tiles on 256 CUs): 264 us whole, 200 + 19 cut; pieces of 12, 20 or 26 slices the same, 40 slower.
 struct Fp8Tile { int bm, bn; float step, fixed; };
 constexpr Fp8Tile FP8_TILES[] = {{256, 256, 1.15f, 6.5f}, {128, 256, 0.86f, 5.0f}, {256, 128, 0.85f, 5.0f}, {128, 128, 0.54f, 5.5f},
                                  {64, 256, 0.63f, 4.5f},  {64, 128, 0.40f, 5.5f},  {32, 256, 0.54f, 3.0f},  {32, 128, 0.38f, 5.0f},
@@ -443,8 +561,14 @@ static bool fp8_tile_ok(int bm, int bn, int kq) {
     if (EPI == EPI_GELU_NEW) return bn == 256 || bn == 128;
     return true;
 }
+constexpr int FP8_PIECE_SLICES = 12;  // a piece covers at least this many slices
+constexpr size_t FP8_SPLIT_BYTES = (size_t)8 * FP8_XCD_CUS * 256 * 256 * 4;  // one 256 x 256 fp32 tile per CU: 64 MiB
+// whether a product could use that workspace at all: K long enough to cut, and about a round of big tiles
+static bool fp8_may_split(long long rows, int K, int N) { return K >= 32 * QB && rows / 256 * ((N + 255) / 256) >= 192; }
+
+// the estimate, the tile and (split) the largest number of pieces: 1 = tiles stay whole
 template <int EPI>
-static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p, double *estimate = nullptr) {
+static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p, double *estimate = nullptr, int *split = nullptr) {
     const int nk = (p.K + QB - 1) / QB, kq = (nk + 3) / 4 * 4;
     const double parts = p.max_rows < p.G ? p.max_rows : p.G;  // groups that can hold rows: half a tile of each is lost
     const Fp8Tile *best = nullptr;
@@ -458,20 +582,30 @@ static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p, double *estimate =
         const double fill = tiles * nk * (t.bm + t.bn) * 128e-6 / 10.5;
         double us = rounds * (nk * t.step + t.fixed);
         if (fill > us) us = fill;
-        if (!best || us < best_t) { best = &t; best_t = us; }
+        int cut = 1;
+        if (EPI == EPI_PLAIN && t.bm == 256 && t.bn == 256 && p.splitk_ws && nk >= 32) {
+            const int n = (int)(tiles / 8) + 1, rm = n % FP8_XCD_CUS;
+            int s = rm ? FP8_XCD_CUS / rm : 1;
+            if (s > nk / FP8_PIECE_SLICES) s = nk / FP8_PIECE_SLICES;
+            const double cut_us = (n / FP8_XCD_CUS) * (nk * t.step + t.fixed) + ((double)nk / s * t.step + t.fixed) + 5.0 + 8 * rm * s * 0.11;
+            if (s >= 2 && cut_us < us) { us = cut_us; cut = s; }
+        }
+        if (!best || us < best_t) { best = &t; best_t = us; if (split) *split = cut; }
     }
     if (estimate) *estimate = best_t;
     return *best;
 }
 
 template <int DT, int EPI>
-static int launch_fp8_gemm(const Fp8GemmParams &p, hipStream_t st) {
+static int launch_fp8_gemm(Fp8GemmParams p, hipStream_t st) {
     int bm, bn;
+    p.split_max = 1;
     const Knobs &k = knobs();
     if (k.tile_bm && fp8_tile_ok<EPI>(k.tile_bm, k.tile_bnw, ((p.K + QB - 1) / QB + 3) / 4 * 4)) {
         bm = k.tile_bm; bn = k.tile_bnw;
+        if (bm == 256 && bn == 256) p.split_max = k.splitk;
     } else {
-        const Fp8Tile &t = choose_fp8_tile<EPI>(p);
+        const Fp8Tile &t = choose_fp8_tile<EPI>(p, nullptr, &p.split_max);
         bm = t.bm; bn = t.bn;
     }
 #define FP8_TILE(M_, N_) if (bm == M_ && bn == N_) return launch_fp8_tile<DT, EPI, M_, N_>(p, st);
@@ -564,8 +698,9 @@ extern "C" int moe_grouped_gemm_fp8_fwd(const void *a, int64_t lda, const void *
 
 extern "C" size_t moe_grouped_linear_fp8_workspace_bytes(int rows, int K) {
     if (rows < 0 || K < 1) return 0;
-    const size_t q = ((size_t)rows * K + 255) & ~(size_t)255;
-    return q + (size_t)rows * (((K + QB - 1) / QB + 3) / 4 * 4);
+    const size_t q = ((size_t)rows * K + 255) & ~(size_t)255, qs = (size_t)rows * (((K + QB - 1) / QB + 3) / 4 * 4);
+    // the K pieces' share: N is not known here, so long K and about a round of big tiles at N = 2048
+    return q + (fp8_may_split(rows, K, 2048) ? ((qs + 255) & ~(size_t)255) + FP8_SPLIT_BYTES : qs);
 }
 
 extern "C" int moe_grouped_linear_fp8_fwd(const void *x, int64_t ldx, const void *w, const void *w_scale, const void *bias,
@@ -584,9 +719,10 @@ extern "C" int moe_grouped_linear_fp8_fwd(const void *x, int64_t ldx, const void
     if (ws_bytes < moe_grouped_linear_fp8_workspace_bytes(rows, K)) return fail(MOE_ERR_WORKSPACE, "%s: workspace %zu bytes too small", fn, ws_bytes);
     if (rows == 0) return 0;
     u8 *q = (u8 *)workspace, *qs = q + (((size_t)rows * K + 255) & ~(size_t)255);
-    const Fp8GemmParams p = plain_params(q, K, qs, ld_as, nullptr, 0, w, w_scale, bias, group_offsets, G, n_experts_local, rows, K, N,
+    Fp8GemmParams p = plain_params(q, K, qs, ld_as, nullptr, 0, w, w_scale, bias, group_offsets, G, n_experts_local, rows, K, N,
                                    zero_tail, out, ldo);
     if ((rc = moe_quantize_rows_fp8(x, ldx, rows, K, q, K, qs, ld_as, dtype, stream))) return rc;
+    if (fp8_may_split(rows, K, 2048)) p.splitk_ws = (float *)(qs + (((size_t)rows * ld_as + 255) & ~(size_t)255));
     return fp8_gemm(p, MOE_EPI_PLAIN, dtype, (hipStream_t)stream);
 }
 
@@ -594,6 +730,7 @@ namespace {
 inline size_t pad256b(size_t b) { return (b + 255) & ~(size_t)255; }
 struct FfnWs {
     u8 *hq, *hs, *aq, *as;
+    float *split;
     long long ld_hs, ld_as;
     size_t total;
 };
@@ -608,6 +745,7 @@ FfnWs carve_ffn(void *ws, int src_rows, int max_rows, int M, int I) {
     r.hs = take((size_t)max_rows * r.ld_hs);
     r.aq = take((size_t)src_rows * M);
     r.as = take((size_t)src_rows * r.ld_as);
+    r.split = fp8_may_split(max_rows, I, M) ? (float *)take(FP8_SPLIT_BYTES) : nullptr;
     r.total = off;
     return r;
 }
@@ -659,5 +797,6 @@ extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int s
     p.n_gated = (n_gated < 0 || n_gated > I) ? I : n_gated;
     if ((rc = fp8_gemm(p, gated ? MOE_EPI_SWIGLU : MOE_EPI_GELU_NEW, dtype, (hipStream_t)stream))) return rc;
     p = plain_params(ws.hq, I, ws.hs, ws.ld_hs, nullptr, 0, w2, w2_scale, b2, group_offsets, G, n_experts_local, max_rows, I, M, 0, y, M);
+    p.splitk_ws = ws.split;
     return fp8_gemm(p, MOE_EPI_PLAIN, dtype, (hipStream_t)stream);
 }

@@ -107,6 +107,30 @@ def test_few_rows(S, K, N, tile):
         assert torch.equal(y.view(S, N // tile, tile), y[:, :tile].unsqueeze(1).expand(S, N // tile, tile))
 
 
+@pytest.mark.parametrize("G,S,K,N,bias", [(1, 6700, 4096, 2560, True), (3, 6854, 5632, 2553, False), (2, 6600, 10240, 2560, True)])
+def test_last_round_cut_along_k(G, S, K, N, bias):
+    """Launches whose last round of 256 x 256 tiles is cut along K (one full round and a few tiles more): every element, ragged
+    groups, rows of no group, an N that rules wide stores out, and the same bits every time."""
+    g = torch.Generator().manual_seed(S)
+    x = _rows(g, S, K, torch.bfloat16)
+    q, s = R.weights(g, G, N, K)
+    b = torch.randn((G, N), generator=g).to(torch.bfloat16) if bias else None
+    offs = torch.tensor([0, S] if G == 1 else [0, S // 3, S - 700, S - 5] if G == 3 else [3, S // 2, S], dtype=torch.int32)
+    gx, gq, gs, gb = x.to(DEV), q.to(DEV), s.to(DEV), b.to(DEV) if bias else None
+
+    def run():
+        return fp8.linear(gx, gq[0], gs[0], gb[0] if bias else None) if G == 1 else fp8.grouped_linear(gx, gq, gs, offs.to(DEV), gb)
+    y = run()
+    xd = R.deq(x).to(DEV)
+    for e in range(G):
+        lo, hi = int(offs[e]), int(offs[e + 1])
+        ref, tol = R.product(xd[lo:hi], R.deq_stored(q[e], s[e]).to(DEV))
+        R.check16(y[lo:hi], (ref + b[e].to(DEV).to(D) if bias else ref).cpu(), tol.cpu(), f"group {e}")
+    assert not bool(y[:int(offs[0])].any()) and not bool(y[int(offs[-1]):].any())
+    for _ in range(2):
+        assert torch.equal(run(), y)
+
+
 @pytest.mark.parametrize("S,K,N", [(1, 64, 16), (37, 208, 144), (300, 512, 272), (70, 1040, 640)])
 def test_linear_input_gradient(S, K, N):
     g = torch.Generator().manual_seed(S + K + N)
