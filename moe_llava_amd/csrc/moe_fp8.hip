@@ -47,7 +47,7 @@ template <int EPI, int BM, int BNW>
 struct FTile {
     static constexpr bool GATED = EPI == EPI_SWIGLU;
     static constexpr bool QOUT = EPI != EPI_PLAIN;            // output quantised for the next product
-    static_assert(BM == 256 || BM == 128 || BM == 64 || BM == 32, "row tile");
+    static_assert(BM == 256 || BM == 192 || BM == 128 || BM == 64 || BM == 32, "row tile");
     static_assert(BNW == 256 || ((BNW == 128 || BNW == 64) && !GATED), "column tile");
     static_assert(!QOUT || (GATED ? BNW / 2 : BNW) % QB == 0, "an output block lies in one tile");
     static constexpr int SLOT = (BM + BNW) * QB;              // bytes of one K slice
@@ -240,9 +240,9 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
     auto load_scales = [&]() {
         const int t2 = tid - 256;
         const int kq_n = (nk + 3) >> 2;
-        const int r = t2 & (BM - 1);
+        const int r = t2 % BM;
         const u8 *src = p.a_scale + src_row(row_begin + r) * p.ld_as;
-        for (int kq = t2 / BM; kq < kq_n; kq += 256 / BM)
+        for (int kq = t2 < 256 / BM * BM ? t2 / BM : kq_n; kq < kq_n; kq += 256 / BM)
             *reinterpret_cast<unsigned *>(lds + T::XS + (kq * BM + r) * 4) = *reinterpret_cast<const unsigned *>(src + kq * 4);
         const u8 *wsb = p.w_scale + (long long)expert * p.ws_expert_stride;
         const int nb = (p.N_out + QB - 1) / QB;
@@ -541,17 +541,17 @@ static int launch_fp8_tile(Fp8GemmParams p, hipStream_t st) {
     return check_launch("fp8_fixup_kernel");
 }
 
-// Tile choice.  One block runs on a CU at a time, so a launch takes ceil(tiles / 256) rounds of (slices * step + fixed);
-// a launch of many rounds is held by the fills instead, tiles * slices * (BM + BNW) * 128 bytes at ~10.5 TB/s from L2.  The
-// constants were measured on one-round launches (K = 5632 and 10240, one group and four; microseconds): they are a CU's time
-// per slice with its fills in flight, and prologue + epilogue.  The smallest estimate is within 5 % of the best of
-// twelve tiles on 36 of 40 swept shapes (100 ... 11264 rows, K 1024 ... 10240, N 1024 ... 5632, 1 to 8 groups) and 21 % off
-// at worst; the 256 x 256 tile alone is up to 3.2 x off there (1408 rows, K 5632, N 2048, 4 groups: 57.9 us against 30.9).
+// Tile choice.  One block runs on a CU at a time, so a launch takes rounds of 256 tiles; a round takes slices * step + fixed.
+// step is a CU's time per slice with its fills in flight, or, when the round's tiles together ask for more than the caches
+// deliver, their (BM + BNW) * 128 bytes per slice at 13 TB/s.  The constants were measured on one-round launches (K = 5632 and
+// 10240, one group and four; microseconds).  The smallest estimate is within 5 % of the best of thirteen tiles on 39 of 44
+// swept shapes (100 ... 11264 rows, K 1024 ... 10240, N 1024 ... 5632, 1 to 8 groups), 1.6 % off on average and 21 % at worst;
+// the 256 x 256 tile alone is up to 3.2 x off there (1408 rows, K 5632, N 2048, 4 groups: 57.9 us against 30.9).
 // With a workspace, the 256 x 256 tile's last round may be cut along K (Fp8Sched): its estimate is then the whole rounds, a
 // piece of the tail, and the pieces written and read back (0.11 us each at 4.7 TB/s, 5 us for the launch).  6854 rows, K
 // 10240, N 2560 (290 tiles on 256 CUs): 264 us whole, 200 + 19 cut; pieces of 12, 20 or 26 slices the same, 40 slower.
 struct Fp8Tile { int bm, bn; float step, fixed; };
-constexpr Fp8Tile FP8_TILES[] = {{256, 256, 1.15f, 6.5f}, {128, 256, 0.86f, 5.0f}, {256, 128, 0.85f, 5.0f}, {128, 128, 0.54f, 5.5f},
+constexpr Fp8Tile FP8_TILES[] = {{256, 256, 1.15f, 6.5f}, {192, 256, 1.0f, 6.0f}, {128, 256, 0.86f, 5.0f}, {256, 128, 0.85f, 5.0f}, {128, 128, 0.54f, 5.5f},
                                  {64, 256, 0.63f, 4.5f},  {64, 128, 0.40f, 5.5f},  {32, 256, 0.54f, 3.0f},  {32, 128, 0.38f, 5.0f},
                                  {32, 64, 0.31f, 5.0f}};
 template <int EPI>
@@ -578,17 +578,18 @@ static const Fp8Tile &choose_fp8_tile(const Fp8GemmParams &p, double *estimate =
         const int nc = EPI == EPI_SWIGLU ? t.bn / 2 : t.bn;
         const double rt = p.G == 1 ? (double)((p.max_rows + t.bm - 1) / t.bm) : ((double)p.max_rows / t.bm + 0.5 * parts) * 1.05;
         const double tiles = rt * ((p.N_out + nc - 1) / nc);
-        const double rounds = (double)(long long)((tiles + 255) / 256);
-        const double fill = tiles * nk * (t.bm + t.bn) * 128e-6 / 10.5;
-        double us = rounds * (nk * t.step + t.fixed);
-        if (fill > us) us = fill;
+        const double slice = (t.bm + t.bn) * 128e-6 / 13.0;    // a tile's fills of a slice at the chip's rate
+        auto round_us = [&](double n, double slices) { return slices * (n * slice > t.step ? n * slice : t.step) + t.fixed; };
+        const int full = (int)(tiles / 256);
+        const double rest = tiles - 256.0 * full;
+        double us = full * round_us(256, nk) + (rest > 0 ? round_us(rest, nk) : 0.0);
         int cut = 1;
         if (EPI == EPI_PLAIN && t.bm == 256 && t.bn == 256 && p.splitk_ws && nk >= 32) {
             const int n = (int)(tiles / 8) + 1, rm = n % FP8_XCD_CUS;
             int s = rm ? FP8_XCD_CUS / rm : 1;
             if (s > nk / FP8_PIECE_SLICES) s = nk / FP8_PIECE_SLICES;
-            const double cut_us = (n / FP8_XCD_CUS) * (nk * t.step + t.fixed) + ((double)nk / s * t.step + t.fixed) + 5.0 + 8 * rm * s * 0.11;
-            if (s >= 2 && cut_us < us) { us = cut_us; cut = s; }
+            const double cut_us = s >= 2 ? (n / FP8_XCD_CUS) * round_us(256, nk) + round_us(8 * rm * s, (double)nk / s) + 5.0 + 8 * rm * s * 0.11 : us;
+            if (cut_us < us) { us = cut_us; cut = s; }
         }
         if (!best || us < best_t) { best = &t; best_t = us; if (split) *split = cut; }
     }
@@ -609,7 +610,7 @@ static int launch_fp8_gemm(Fp8GemmParams p, hipStream_t st) {
         bm = t.bm; bn = t.bn;
     }
 #define FP8_TILE(M_, N_) if (bm == M_ && bn == N_) return launch_fp8_tile<DT, EPI, M_, N_>(p, st);
-    FP8_TILE(256, 256) FP8_TILE(128, 256) FP8_TILE(64, 256) FP8_TILE(32, 256)
+    FP8_TILE(256, 256) FP8_TILE(192, 256) FP8_TILE(128, 256) FP8_TILE(64, 256) FP8_TILE(32, 256)
     if constexpr (EPI != EPI_SWIGLU) { FP8_TILE(256, 128) FP8_TILE(128, 128) FP8_TILE(64, 128) FP8_TILE(32, 128) }
     if constexpr (EPI == EPI_PLAIN) { FP8_TILE(32, 64) }
 #undef FP8_TILE
