@@ -602,7 +602,9 @@ static int launch_fp8_gemm(Fp8GemmParams p, hipStream_t st) {
     int bm, bn;
     p.split_max = 1;
     const Knobs &k = knobs();
-    if (k.tile_bm && fp8_tile_ok<EPI>(k.tile_bm, k.tile_bnw, ((p.K + QB - 1) / QB + 3) / 4 * 4)) {
+    bool forced = false;                                       // MOE_GEMM_TILE, where it names a tile of this table
+    for (const Fp8Tile &t : FP8_TILES) forced |= t.bm == k.tile_bm && t.bn == k.tile_bnw;
+    if (forced && fp8_tile_ok<EPI>(k.tile_bm, k.tile_bnw, ((p.K + QB - 1) / QB + 3) / 4 * 4)) {
         bm = k.tile_bm; bn = k.tile_bnw;
         if (bm == 256 && bn == 256) p.split_max = k.splitk;
     } else {

@@ -51,6 +51,9 @@ class GraphedMoE:
         self.x = example.detach().clone()
         self.graph = torch.cuda.CUDAGraph()
         gate.__dict__["noise_seed_dev"] = self.seed_dev
+        # a decode step's buffers belong to its plan; the captured step gets plans of its own, or two graphs of one layer
+        # (captured on the same stream) would write the same buffers when they are replayed on two streams
+        plans = layer.__dict__.pop("_decode_plans", None)
         try:
             with torch.no_grad():
                 side = torch.cuda.Stream(device=dev)
@@ -63,9 +66,16 @@ class GraphedMoE:
                     self.out = self._forward()
         finally:
             gate.__dict__.pop("noise_seed_dev", None)
+            self._plans = layer.__dict__.pop("_decode_plans", None)
+            if plans is not None:
+                layer.__dict__["_decode_plans"] = plans
         # 8-bit experts: the graph reads this copy of them; the reference keeps it alive, __call__ keeps it up to date
-        self._fp8 = layer.experts.packed_fp8(dev) if layer.experts.fp8 else None
+        self._fp8, self._n_gated = self._form(dev)
         self.routing = layer.last_routing      # static routing arrays of the captured step (overwritten per replay)
+
+    def _form(self, dev):
+        experts = self.layer.experts
+        return (experts.packed_fp8(dev), experts.n_gated) if experts.fp8 else (None, None)
 
     def _forward(self):
         res = self.moe(self.x)
@@ -77,9 +87,10 @@ class GraphedMoE:
         if x.shape != self.x.shape or x.dtype != self.x.dtype or x.device != self.x.device:
             raise ValueError(f"GraphedMoE: captured for {tuple(self.x.shape)} {self.x.dtype} on {self.x.device}, got "
                              f"{tuple(x.shape)} {x.dtype} on {x.device}")
-        experts = self.layer.experts
-        if (experts.packed_fp8(x.device) if experts.fp8 else None) is not self._fp8:
-            raise ValueError("GraphedMoE: captured on another form of the experts (16-bit, or another 8-bit copy): capture again")
+        fp8, n_gated = self._form(x.device)
+        if fp8 is not self._fp8 or n_gated != self._n_gated:
+            raise ValueError("GraphedMoE: captured on another form of the experts (16-bit, another 8-bit copy, or another "
+                             "number of gated channels): capture again")
         self.x.copy_(x)
         self.graph.replay()
         return self.out

@@ -69,21 +69,30 @@ class MoE(nn.Module):
         self.deepspeed_moe.experts.quantize_fp8(on)
         return self
 
-    def forward_normed(self, hidden_states: Tensor, residual: Tensor, norm: nn.Module, used_token: Optional[Tensor] = None):
-        """The step of a pre-norm decoder layer in front of and through the block: ``s = hidden_states + residual``,
+    def forward_normed(self, hidden_states: Tensor, residual: Optional[Tensor], norm: nn.Module, used_token: Optional[Tensor] = None):
+        """The step of a pre-norm decoder layer in front of and through the block: ``s = hidden_states + residual`` (or, with
+        ``residual`` None, ``hidden_states``),
         ``forward(rms_norm(s))``.  Returns ``(output, l_aux, exp_counts, s)``; the layer's output is ``s + output``.  ``norm``:
-        a module with ``weight`` and ``eps`` (or ``variance_epsilon``).  With 8-bit experts the norm's launch writes the rows in
-        8 bits beside the 16-bit rows that the gate reads, otherwise this is ``norm.add_rms_norm`` and ``forward``."""
+        a root-mean-square norm with ``weight`` and ``eps`` (or ``variance_epsilon``).  With 8-bit experts the norm's launch
+        writes the rows in 8 bits beside the 16-bit rows that the gate reads, otherwise, and for a subclass with a ``forward``
+        of its own or a module with hooks, this is ``norm.add_rms_norm`` and ``forward``."""
         from . import norm as norm_ops
+        from .sharded_moe import module_has_hooks
+        if isinstance(norm, nn.LayerNorm) or getattr(norm, "bias", None) is not None:
+            raise TypeError(f"forward_normed: {type(norm).__name__} is no root-mean-square norm with a weight only")
         eps = getattr(norm, "eps", None)
         if eps is None:
             eps = norm.variance_epsilon
         layer = self.deepspeed_moe
-        if not self.use_residual and layer.takes_fp8_rows(hidden_states, used_token):
+        if not self.use_residual and type(self).forward is MoE.forward and not module_has_hooks(self) \
+                and layer.takes_fp8_rows(hidden_states, used_token):
             rows, y, s = norm_ops.add_rms_norm_fp8(hidden_states, residual, norm.weight, eps)
             out = layer(y, used_token, rows)
             return out, layer.l_aux, layer.exp_counts, s
-        y, s = norm_ops.add_rms_norm(hidden_states, residual, norm.weight, eps)
+        if residual is None:
+            y, s = norm_ops.rms_norm(hidden_states, norm.weight, eps), hidden_states
+        else:
+            y, s = norm_ops.add_rms_norm(hidden_states, residual, norm.weight, eps)
         out, l_aux, exp_counts = self(y, used_token)
         return out, l_aux, exp_counts, s
 

@@ -516,7 +516,7 @@ class MOELayer(nn.Module):
             plans = d["_decode_plans"] = {}
         wgw = gate.wg.weight
         key = (experts.fp8, S, x.dtype, x.device.index, st, gate.training, wgw.data_ptr(), wgw.dtype, gate.capacity_factor,
-               gate.eval_capacity_factor, gate.min_capacity, gate.drop_tokens, gate.top2_2nd_expert_sampling)
+               gate.eval_capacity_factor, gate.min_capacity, gate.drop_tokens, gate.top2_2nd_expert_sampling, experts.n_gated)
         plan = plans.get(key)
         if plan is None or plan.packed is not packed:
             if len(plans) >= 32:

@@ -104,3 +104,15 @@ def test_reference_rounds_like_the_type():
     assert torch.equal(R.e4m3(v), v.to(torch.float32).to(R.E4M3).to(torch.float32).to(torch.float64))
     top = torch.tensor([0.0, 448.0, 448.0001, 1.75, 1.7500001, 896.0, 1e-40], dtype=torch.float64)
     assert R.scale_byte(top).tolist() == [1, 127, 128, 119, 120, 128, 1]
+
+
+def test_forward_normed_refuses_other_norms():
+    """A LayerNorm has a weight and an eps as well, but is another norm."""
+    import moe_llava_amd
+    from tests.expert_mlps import StableLMMLP
+    moe = moe_llava_amd.MoE(64, StableLMMLP(64, 64), num_experts=2, k=2)
+    x = torch.zeros((2, 64))
+    with pytest.raises(TypeError):
+        moe.forward_normed(x, None, torch.nn.LayerNorm(64))
+    with pytest.raises(TypeError):
+        moe.forward_normed(x, None, torch.nn.LayerNorm(64, elementwise_affine=False))

@@ -7,7 +7,7 @@ import moe_llava_amd
 from moe_llava_amd import fp8, norm
 from moe_llava_amd.graph import GraphedMoE
 from tests import _fp8_ref as R
-from tests.expert_mlps import PhiMLP, StableLMMLP
+from tests.expert_mlps import PhiMLP, RePaMLP, StableLMMLP
 from tests.test_gpu_fp8 import _check_ffn, _ffn_ref
 
 pytestmark = pytest.mark.gpu
@@ -193,3 +193,152 @@ def test_refusals():
             moe.deepspeed_moe.experts(torch.zeros((1, 4, 2, 256), dtype=torch.bfloat16, device=DEV))
     with pytest.raises(NotImplementedError):
         moe_llava_amd.MoE(256, StableLMMLP(256, 320).to(torch.bfloat16), num_experts=4, ep_size=2, k=2).quantize_experts()
+
+
+@pytest.mark.parametrize("S", [5, 130])
+def test_masked_experts_follow_their_mask(S):
+    """Experts with a channel mask: the number of gated channels can change between two calls of the same size."""
+    torch.manual_seed(0)
+    moe = moe_llava_amd.MoE(256, RePaMLP(256, 320).to(torch.bfloat16), num_experts=4, k=2, eval_capacity_factor=2.0,
+                            min_capacity=0, top2_2nd_expert_sampling=False).to(DEV)
+    with torch.no_grad():
+        for n, p in moe.named_parameters():
+            p.copy_((torch.randn(p.shape) * (0.3 if "wg" in n else 0.08)).to(p.dtype))
+    moe = moe.to(torch.bfloat16).eval().quantize_experts()
+    x = _x(S, 256)
+    specs = moe.deepspeed_moe.experts
+    with torch.no_grad():
+        seen = []
+        for ratio in (1.0, 0.5, 0.25, 1.0):
+            for e in specs.deepspeed_experts:
+                e.adjust_gated_ratio(ratio)
+            out = moe(x)[0].clone()
+            lay, r = moe.deepspeed_moe, moe.deepspeed_moe.last_routing
+            ng = int(320 * ratio) if ratio < 1 else -1
+            want = fp8.block_top2(x, lay.gate.wg.weight, r.capacity, None, 0, True, specs.packed_fp8(x.device), ng)[0]
+            assert torch.equal(out, want)
+            seen.append(out)
+        assert torch.equal(seen[0], seen[3]) and not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+        if S == 5:
+            g = GraphedMoE(moe, x)
+            assert torch.equal(g(x)[0], seen[0])
+            for e in specs.deepspeed_experts:
+                e.adjust_gated_ratio(0.5)
+            with pytest.raises(ValueError):
+                g(x)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_two_graphs_of_one_layer_share_no_buffer(eight):
+    moe = _moe()
+    if eight:
+        moe.quantize_experts()
+    a, b = _x(8, 256, seed=5), _x(8, 256, seed=6)
+    g1, g2 = GraphedMoE(moe, a), GraphedMoE(moe, a)
+    with torch.no_grad():
+        ra = [t.clone() for t in moe(a)[:3]]
+        rb = [t.clone() for t in moe(b)[:3]]
+        for _ in range(3):
+            o1 = g1(a)
+            torch.cuda.synchronize()
+            o2 = g2(b)
+            torch.cuda.synchronize()
+            moe(a)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(o1, ra)) and all(torch.equal(p, q) for p, q in zip(o2, rb))
+
+
+def test_a_forced_tile_that_the_products_lack(monkeypatch):
+    """A tile forced for the 16-bit products that the 8-bit ones do not have leaves those to their rule."""
+    from moe_llava_amd import ops
+    moe = _moe().quantize_experts()
+    x = _x(200, 256)
+    with torch.no_grad():
+        want = moe(x)[0].clone()
+        try:
+            monkeypatch.setenv("MOE_GEMM_TILE", "256,64")
+            ops.reload_knobs()
+            assert torch.equal(moe(x)[0], want)
+        finally:
+            monkeypatch.delenv("MOE_GEMM_TILE")
+            ops.reload_knobs()
+
+
+def test_flattened_parameters_are_followed():
+    """Parameters that are views into somebody else's buffer: copied and quantised for each call."""
+    moe, x = _moe(), _x(24, 256)
+    ps = list(moe.deepspeed_moe.experts.parameters())
+    flat = torch.cat([p.detach().reshape(-1) for p in ps])
+    at = 0
+    for p in ps:
+        p.data = flat[at:at + p.numel()].view(p.shape)
+        at += p.numel()
+    same = _moe().quantize_experts()
+    with torch.no_grad(), pytest.warns(UserWarning):
+        moe.quantize_experts()
+        a = moe(x)[0].clone()
+    with torch.no_grad():
+        assert torch.equal(a, same(x)[0])
+        flat.mul_(0)
+        assert not bool(moe(x)[0].any())
+
+
+def test_two_streams_and_a_second_module():
+    """The same layer on two streams, and another layer between: every call its own buffers."""
+    m1, m2 = _moe().quantize_experts(), _moe(form="gelu_new", I=448).quantize_experts()
+    x1, x2 = _x(32, 256, seed=8), _x(600, 256, seed=9)
+    st = [torch.cuda.Stream() for _ in range(2)]
+    with torch.no_grad():
+        want = [m(x)[0].clone() for m, x in ((m1, x1), (m2, x2), (m2, x1), (m1, x2))]
+        torch.cuda.synchronize()
+        got = []
+        for k in range(6):
+            with torch.cuda.stream(st[k % 2]):
+                got.append([m(x)[0] for m, x in ((m1, x1), (m2, x2), (m2, x1), (m1, x2))])
+        torch.cuda.synchronize()
+        for row in got:
+            assert all(torch.equal(a, b) for a, b in zip(row, want))
+
+
+@pytest.mark.parametrize("S", [3, 90])
+def test_normed_block_shapes_and_fallbacks(S):
+    """forward_normed without a residual, on rows with a stride, on 16-bit experts, top-1 and a width of 8-bit tails."""
+    for M, kw in ((320, {}), (256, dict(k=1, use_rts=False))):
+        moe = _moe(M=M, **kw).quantize_experts()
+        nm = norm.RMSNorm(M, eps=1e-5, dtype=torch.bfloat16, device=DEV)
+        x = _x(S, 2 * M, seed=12)[:, :M]
+        with torch.no_grad():
+            out, la, ec, s = moe.forward_normed(x, None, nm)
+            la, ec = la.clone(), ec.clone()
+            assert torch.equal(s, x)
+            if not kw:                       # the norm's launch quantises its fp32 values, not the rounded 16-bit ones
+                lay = moe.deepspeed_moe
+                rows, y, _ = norm.add_rms_norm_fp8(x, None, nm.weight, 1e-5)
+                want = fp8.block_top2(y, lay.gate.wg.weight, lay.last_routing.capacity, None, 0, True,
+                                      lay.experts.packed_fp8(x.device), -1, None, rows)[0]
+                assert torch.equal(out, want)
+            want = moe(nm(x))
+            assert (not kw or torch.equal(out, want[0])) and torch.equal(la, want[1]) and torch.equal(ec, want[2])
+            moe.quantize_experts(False)
+            out = moe.forward_normed(x, None, nm)[0]
+            assert torch.equal(out, moe(nm(x))[0])
+
+
+def test_normed_block_keeps_what_is_around_the_forward():
+    """A subclass with a forward of its own and hooks on the module are not passed by."""
+    class Scaled(moe_llava_amd.MoE):
+        def forward(self, x, *args, **kwargs):
+            out, l_aux, counts = super().forward(x, *args, **kwargs)
+            return out * 2, l_aux, counts
+
+    moe = _moe().quantize_experts()
+    nm = norm.RMSNorm(256, eps=1e-5, dtype=torch.bfloat16, device=DEV)
+    x, r = _x(20, 256, seed=3), _x(20, 256, seed=4)
+    with torch.no_grad():
+        want = moe(norm.add_rms_norm(x, r, nm.weight, 1e-5)[0])[0].clone()
+        seen = []
+        h = moe.register_forward_hook(lambda m, i, o: seen.append(1))
+        assert torch.equal(moe.forward_normed(x, r, nm)[0], want) and seen
+        h.remove()
+        moe.__class__ = Scaled
+        assert torch.equal(moe.forward_normed(x, r, nm)[0], want * 2)
