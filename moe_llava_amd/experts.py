@@ -266,7 +266,8 @@ class Experts(nn.Module):
     def quantize_fp8(self, on: bool = True) -> None:
         """Run the experts in 8 bits (``fp8.expert_ffn``) from the next inference call on, or in 16 bits again.  The 16-bit
         parameters stay: checkpoints are unchanged, and the 8-bit copy is made again when one of them was replaced or
-        changed in place (a write through ``.data`` is not seen: call this again after one)."""
+        changed in place (a write through ``.data`` is not seen: call this again after one).  Parameters made in inference
+        mode keep no version: they are quantised again on every call."""
         self.fp8 = bool(on)
         self._fp8 = None
 
@@ -281,7 +282,7 @@ class Experts(nn.Module):
         """(act, w1, w1_scale, b1|None, w2, w2_scale, b2|None) of the 8-bit experts, quantised from ``packed()``.  When the
         16-bit weights change, the same tensors are filled again: a captured graph that reads them stays valid."""
         cur = self._fp8
-        if cur is not None and cur[0] == device and self.packed_unchanged() is not None \
+        if cur is not None and cur[0] == device and cur[1] is not None and self.packed_unchanged() is not None \
                 and cur[1] == self._versions([c[2] for c in self._fast[0]]):
             return cur[2]
         from . import fp8
@@ -290,7 +291,7 @@ class Experts(nn.Module):
         params = self._params(specs)
         self._remember_fast(specs, (act, w1, b1, w2, b2))
         versions = self._versions(params)
-        if cur is not None and cur[0] == device and cur[1] == versions and cur[3] == self._ptrs and not self._external:
+        if cur is not None and cur[0] == device and versions is not None and cur[1] == versions and cur[3] == self._ptrs and not self._external:
             return cur[2]
         nproj = len(specs[0].fc1)
         old = cur[2] if cur is not None and cur[0] == device else None

@@ -26,6 +26,7 @@ BLOCK = 128
 E4M3 = torch.float8_e4m3fn
 E8M0 = torch.float8_e8m0fnu
 MAX_K = 65536            # columns of a product's operands
+MAX_ROWS = 2 ** 31 - 1   # row counts and matrix dimensions are 32-bit in the library
 _ACTS = {"swiglu": ops.ACT_SWIGLU, "gelu_new": ops.ACT_GELU_NEW, ops.ACT_SWIGLU: ops.ACT_SWIGLU,
          ops.ACT_GELU_NEW: ops.ACT_GELU_NEW}
 
@@ -67,12 +68,14 @@ def _half_rows(x: Tensor, name: str) -> Tensor:
     if x.dtype not in ops.HALF_DTYPES:
         raise TypeError(f"{name}: expected bf16 or fp16, got {x.dtype}")
     d = x.dim()
-    if d == 2 and x.is_contiguous():
-        return x
     if d < 1:
         raise ValueError(f"{name}: expected at least one dimension")
     if d != 2:
         x = x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(x.shape[:-1].numel(), x.shape[-1])
+    if x.shape[0] > MAX_ROWS:
+        raise ValueError(f"{name}: {x.shape[0]} rows: at most {MAX_ROWS}")
+    if d == 2 and x.is_contiguous():
+        return x
     if x.shape[1] > 1 and x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         x = x.contiguous()                  # transposed, or rows that overlap (an expanded row)
     return x
@@ -85,6 +88,8 @@ def _check_rows(a: Fp8Rows, name: str) -> Fp8Rows:
     if q.dtype != E4M3 or sc.dtype != E8M0 or q.dim() != 2 or sc.dim() != 2:
         raise TypeError(f"{name}: expected e4m3 rows [S, K] and e8m0 scales [S, ceil(K/128)]")
     S, K = q.shape
+    if S > MAX_ROWS:
+        raise ValueError(f"{name}: {S} rows: at most {MAX_ROWS}")
     if tuple(sc.shape) != (S, _blocks(K)) or sc.device != q.device:
         raise ValueError(f"{name}: scales {tuple(sc.shape)} on {sc.device} do not match rows {tuple(q.shape)} on {q.device}")
     if q.stride(1) != 1 or (S > 1 and (q.stride(0) % 16 or q.stride(0) < K)) or q.data_ptr() % 16:
@@ -177,6 +182,8 @@ def quantize_weight(w: Tensor, projections: int = 1, out=None) -> Tuple[Tensor, 
         w = w.clone()
     n, k = w.shape[-2] // projections, w.shape[-1]
     batch = w.numel() // (n * k)
+    if max(batch, n, k) > MAX_ROWS:
+        raise ValueError(f"w: {tuple(w.shape)}: dimensions of at most {MAX_ROWS}")
     shape_s = tuple(w.shape[:-2]) + (projections * _blocks(n), _blocks(k))
     if out is None:
         q = torch.empty(w.shape, dtype=E4M3, device=w.device)
@@ -190,7 +197,15 @@ def quantize_weight(w: Tensor, projections: int = 1, out=None) -> Tuple[Tensor, 
         rc = _lib.load().moe_quantize_blocks_fp8(w.data_ptr(), batch, n, k, q.data_ptr(), sc.data_ptr(), ops._dt(w),
                                                  _stream(w.device.index))
     _lib.check(rc, "moe_quantize_blocks_fp8")
+    if out is not None:                     # the library's writes are invisible to autograd: a graph that saved them must see
+        torch.autograd.graph.increment_version([t for t in (q, sc) if not t.is_inference()])
     return q, sc
+
+
+def _frozen(*ts) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise NotImplementedError("8-bit experts are frozen: weights, scales and biases with requires_grad are not supported "
+                                  "(torch.no_grad() runs them)")
 
 
 # ------------------------------------------------------------------------------------------------ products
@@ -284,15 +299,12 @@ def _linear(x, w: Tensor, ws: Tensor, bias: Optional[Tensor], offs: Optional[Ten
         if not 2 <= offs.numel() <= 4097:
             raise ValueError("group_offsets needs 2 to 4097 entries")
     E = E or 1
+    _frozen(w, ws, bias)
     if rows is not None:
         return _gemm(rows, w, ws, bias, offs, E, N, K, dtype, grouped)
-    grad = False
-    if torch.is_grad_enabled():
-        if bias is not None and bias.requires_grad:
-            raise NotImplementedError("fp8 products are for frozen weights: bias.requires_grad is not supported")
-        grad = x.requires_grad
-        if grad and (N % 16 or N > MAX_K):
-            raise NotImplementedError(f"the input gradient needs N % 16 == 0 and N <= {MAX_K} (N={N})")
+    grad = torch.is_grad_enabled() and x.requires_grad
+    if grad and (N % 16 or N > MAX_K):
+        raise NotImplementedError(f"the input gradient needs N % 16 == 0 and N <= {MAX_K} (N={N})")
     y = (_LinearFn.apply if grad else _linear16)(x2, w, ws, bias, offs, E, N, K)
     return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (N,))
 
@@ -358,9 +370,10 @@ def expert_ffn(act, x: Union[Tensor, Fp8Rows], w1: Tensor, w1_scale: Tensor, w2:
         _check_bias(b1, "b1", (E, parts * I), dtype, dev)
     if b2 is not None:
         _check_bias(b2, "b2", (E, M), dtype, dev)
+    _frozen(w1, w1_scale, b1, w2, w2_scale, b2)
     _check_index(group_offsets, "group_offsets", dev)
     G = group_offsets.numel() - 1
-    if not 1 <= G <= 4096 or max_rows < 0:
+    if not 1 <= G <= 4096 or not 0 <= max_rows <= MAX_ROWS:
         raise ValueError("group_offsets needs 2 to 4097 entries, max_rows >= 0")
     if gather is not None:
         _check_index(gather, "gather", dev)

@@ -254,7 +254,8 @@ class _DecodePlan:
                 q.xq, q.ld_xq, q.xq_scale, q.ld_xs = fp8.row_pointers(rows8, self.S, self.M, self.dev)
             else:
                 q.xq, q.ld_xq, q.xq_scale, q.ld_xs = None, 0, None, 0
-            rc = self.fn(self.ref, self.qref)
+            with ops._on(self.dev):
+                rc = self.fn(self.ref, self.qref)
         else:
             rc = self.fn(self.ref)
         if rc:

@@ -448,3 +448,49 @@ def test_refusals_on_the_gpu():
             bad()
     with pytest.raises(NotImplementedError):
         fp8.expert_ffn("swiglu", x.clone().requires_grad_(True), q1, s1, q2, s2, offs, 8)
+
+
+def test_groups_without_rows():
+    """Every group empty: rows of no group are 0, and get no gradient."""
+    g = torch.Generator().manual_seed(4)
+    q, s = (t.to(DEV) for t in R.weights(g, 3, 64, 128))
+    for S in (1, 40, 700):
+        x = _rows(g, S, 128, torch.bfloat16).to(DEV).requires_grad_(True)
+        for at in (0, S // 2, S):
+            offs = torch.full((4,), at, dtype=torch.int32, device=DEV)
+            y = fp8.grouped_linear(x, q, s, offs)
+            dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+            assert not bool(y.any()) and not bool(dx.any()) and y.shape == (S, 64)
+
+
+def test_refilled_weights_are_seen_by_a_saved_graph():
+    """Weights that are quantised again between a forward and its backward pass: refused, like any in-place change."""
+    g = torch.Generator().manual_seed(5)
+    w = torch.randn((64, 128), generator=g).to(torch.bfloat16).to(DEV)
+    q, s = fp8.quantize_weight(w)
+    x = _rows(g, 8, 128, torch.bfloat16).to(DEV).requires_grad_(True)
+    y = fp8.linear(x, q, s)
+    fp8.quantize_weight(w * 2, out=(q, s))
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+    with torch.inference_mode():
+        qi, si = fp8.quantize_weight(w)
+        fp8.quantize_weight(w, out=(qi, si))
+
+
+def test_refusals_of_trainable_weights_and_too_many_rows():
+    g = torch.Generator().manual_seed(6)
+    q, s = (t.to(DEV) for t in R.weights(g, 2, 64, 128))
+    x = _rows(g, 8, 128, torch.bfloat16).to(DEV)
+    b = torch.zeros(64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    with pytest.raises(NotImplementedError):
+        fp8.linear(fp8.quantize_rows(x), q[0], s[0], b)
+    with torch.no_grad():
+        fp8.linear(fp8.quantize_rows(x), q[0], s[0], b)
+    q1, s1 = (t.to(DEV) for t in R.weights(g, 2, 32, 128, 2))
+    q2, s2 = (t.to(DEV) for t in R.weights(g, 2, 128, 32))
+    offs = torch.tensor([0, 4, 8], dtype=torch.int32, device=DEV)
+    with pytest.raises(NotImplementedError):
+        fp8.expert_ffn("swiglu", x, q1, s1, q2, s2, offs, 8, b2=torch.zeros((2, 128), dtype=torch.bfloat16, device=DEV, requires_grad=True))
+    with pytest.raises(ValueError):
+        fp8.quantize_rows(x[:1].expand(2 ** 31, 128))

@@ -342,3 +342,15 @@ def test_normed_block_keeps_what_is_around_the_forward():
         h.remove()
         moe.__class__ = Scaled
         assert torch.equal(moe.forward_normed(x, r, nm)[0], want * 2)
+
+
+@pytest.mark.parametrize("S", [8, 100])
+def test_parameters_made_in_inference_mode_are_followed(S):
+    """Such parameters keep no version: a change in place is found because they are quantised for every call."""
+    with torch.inference_mode():
+        moe = _moe().quantize_experts()
+        x = _x(S, 256)
+        a = moe(x)[0].clone()
+        for e in moe.deepspeed_moe.experts.deepspeed_experts:
+            e.down_proj.weight.mul_(2)
+        assert torch.equal(moe(x)[0], (a.float() * 2).to(a.dtype))

@@ -229,3 +229,27 @@ def test_refusals_on_the_gpu():
         norm.add_rms_norm_fp8(x.clone().requires_grad_(True), r, w)
     with pytest.raises(_lib.MoEKernelError):
         norm.rms_norm(x.cpu(), w)
+
+
+def test_gradients_of_both_inputs_are_their_own():
+    """x and residual have the same gradient, but neither owns the other's; one leaf in both places gets it twice."""
+    x, r, w = (t.to(DEV) for t in _data(9, 264, torch.bfloat16, 6))
+    xg, rg = x.clone().requires_grad_(True), r.clone().requires_grad_(True)
+    y, s = norm.add_rms_norm(xg, rg, w)
+    (y.float().sum() + s.float().sum()).backward()
+    assert torch.equal(xg.grad, rg.grad) and xg.grad.data_ptr() != rg.grad.data_ptr()
+    keep = rg.grad.clone()
+    xg.grad.zero_()
+    assert torch.equal(rg.grad, keep)
+    both = x.clone().requires_grad_(True)
+    y, s = norm.add_rms_norm(both, both, w)
+    d1, = torch.autograd.grad(y.float().sum(), both, retain_graph=True)
+    xa, xb = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    da, db = torch.autograd.grad(norm.add_rms_norm(xa, xb, w)[0].float().sum(), (xa, xb))
+    assert torch.equal(d1, da + db)
+    # the new stream is saved for the backward pass: changing it in place is refused
+    y, s = norm.add_rms_norm(xg, rg, w)
+    with torch.no_grad():
+        s.add_(1)
+    with pytest.raises(RuntimeError):
+        y.float().sum().backward()
