@@ -18,8 +18,6 @@
 
 namespace moe {
 
-
-
 constexpr int FTHREADS = 512;
 constexpr int FLW = 4;                 // loader waves (one per SIMD)
 constexpr int FP8_STRIP = 28672;       // LDS bytes for the rows' scales of a tile
@@ -533,7 +531,7 @@ static int launch_fp8_tile(Fp8GemmParams p, hipStream_t st) {
     constexpr bool SPLITS = EPI == EPI_PLAIN && BM == 256 && BNW == 256;
     if (!SPLITS || p.split_max < 2) p.splitk_ws = nullptr;
     const long long grid = (rt * p.col_tiles + 7) / 8 * 8 + (p.zero_tail ? 8 : 0) + (p.splitk_ws ? 8 * FP8_XCD_CUS : 0);
-    if (grid > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "fp8 product: too many tiles (%lld)", grid);
+    if (!grid_fits(grid, FTHREADS)) return fail(MOE_ERR_SHAPE, "fp8 product: too many tiles (%lld)", grid);
     hipLaunchKernelGGL((fp8_gemm_kernel<DT, EPI, BM, BNW>), dim3((unsigned)grid), dim3(FTHREADS), 0, st, p);
     int rc = check_launch("fp8_gemm_kernel");
     if (rc || !p.splitk_ws) return rc;

@@ -150,7 +150,7 @@ int launch_fp8_few(const Fp8GemmParams &p0, hipStream_t st) {
     const int nw = active * ((p.N_out + 31) / 32) >= 256 ? 2 : 1;
     p.col_tiles = (p.N_out + 16 * nw - 1) / (16 * nw);
     const long long grid = (long long)p.G * p.col_tiles;
-    if (grid > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "fp8 product: grid too large");
+    if (!grid_fits(grid, 512)) return fail(MOE_ERR_SHAPE, "fp8 product: grid too large");
     // waves per block: about 16 wave-tasks per CU, at least one block of K each
     const int nk = (p.K + QB - 1) / QB;
     int ks = 8;

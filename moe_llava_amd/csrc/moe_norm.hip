@@ -491,7 +491,7 @@ extern "C" int moe_quantize_rows_fp8(const void *x, int64_t ldx, int S, int M, v
     if (!even2(x) || (reinterpret_cast<uintptr_t>(q) & 7)) return fail(MOE_ERR_ALIGN, "%s: x must be 2-byte, q 8-byte aligned", fn);
     if (S == 0) return 0;
     const long long n = ((long long)S * ((M + QB - 1) / QB) + 15) / 16;
-    if (n > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);
+    if (!grid_fits(n, 256)) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);
     const bool vec = aligned16(x) && (ldx & 7) == 0;
     const dim3 g((unsigned)n), b(256);
     hipStream_t st = (hipStream_t)stream;
@@ -509,7 +509,7 @@ extern "C" int moe_quantize_blocks_fp8(const void *w, int batch, int n, int k, v
     if (batch < 1 || n < 1 || k < 16 || (k & 15)) return fail(MOE_ERR_SHAPE, "%s: need batch >= 1, n >= 1, k %% 16 == 0 (%d, %d, %d)", fn, batch, n, k);
     if (!aligned16(w) || (reinterpret_cast<uintptr_t>(q) & 7)) return fail(MOE_ERR_ALIGN, "%s: w must be 16-byte, q 8-byte aligned", fn);
     const long long g = (long long)batch * ((n + QB - 1) / QB) * ((k + QB - 1) / QB);
-    if (g > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);
+    if (!grid_fits(g, 256)) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);
     if (dtype == MOE_DTYPE_F16)
         hipLaunchKernelGGL((quantize_blocks_kernel<DT_F16>), dim3((unsigned)g), dim3(256), 0, (hipStream_t)stream, (const bf16_t *)w, n, k, (u8 *)q, (u8 *)scale);
     else
@@ -524,7 +524,7 @@ extern "C" int moe_transpose_blocks_fp8(const void *w, const void *scale, int ba
     if (batch < 1 || n < 16 || (n & 15) || k < 16 || (k & 15)) return fail(MOE_ERR_SHAPE, "%s: need n %% 16 == 0 and k %% 16 == 0 (%d, %d, %d)", fn, batch, n, k);
     if (!aligned16(w) || !aligned16(wt)) return fail(MOE_ERR_ALIGN, "%s: weights must be 16-byte aligned", fn);
     const long long g = (long long)batch * ((n + 63) / 64) * ((k + 63) / 64);
-    if (g > 0x7fffffffLL) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);
+    if (!grid_fits(g, 256)) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);
     hipLaunchKernelGGL(transpose_fp8_kernel, dim3((unsigned)g), dim3(256), 0, (hipStream_t)stream, (const u8 *)w, (const u8 *)scale, n, k, (u8 *)wt, (u8 *)scale_t);
     return check_launch("transpose_fp8_kernel");
 }

@@ -494,3 +494,49 @@ def test_refusals_of_trainable_weights_and_too_many_rows():
         fp8.expert_ffn("swiglu", x, q1, s1, q2, s2, offs, 8, b2=torch.zeros((2, 128), dtype=torch.bfloat16, device=DEV, requires_grad=True))
     with pytest.raises(ValueError):
         fp8.quantize_rows(x[:1].expand(2 ** 31, 128))
+
+
+def test_offsets_past_32_bits_in_rows():
+    """More than 2^32 elements of rows and of output: every copy of the same 1024 rows gets the same result."""
+    S, K, N, P = 2 ** 21 + 5, 2064, 2064, 1024
+    g = torch.Generator().manual_seed(9)
+    base = _rows(g, P, K, torch.bfloat16).to(DEV)
+    q, s = R.weights(g, 1, N, K)
+    q, s = q[0].to(DEV), s[0].to(DEV)
+    x = base.repeat(S // P + 1, 1)[:S]
+    y = fp8.linear(x, q, s)                                  # 17 blocks of K: no tile is cut along K
+    assert torch.equal(y[:S // P * P].view(-1, P, N), y[:P].expand(S // P, P, N)) and torch.equal(y[S // P * P:], y[:S % P])
+    ref, tol = R.product(R.deq(base[:64].cpu()), R.deq_stored(q.cpu(), s.cpu()))
+    R.check16(y[-69:-5], R.product(R.deq(x[-69:-5].cpu()), R.deq_stored(q.cpu(), s.cpu()))[0], tol.amax(), "last rows")
+    R.check16(y[:64], ref, tol, "first rows")
+    del x
+    offs = torch.tensor([0, 7, S - 3], dtype=torch.int32, device=DEV)
+    y.fill_(5.0)
+    z = fp8.grouped_linear(y, torch.stack([q, q]), torch.stack([s, s]), offs)     # equal rows in, equal rows out, the tail 0
+    assert not bool(z[-3:].any()) and torch.equal(z[-4], z[0]) and bool((z[:-3] == z[0]).all())
+
+
+def test_offsets_past_31_bits_in_weights():
+    """A weight of 2^32 elements (quantised, read by both kinds of product, transposed): its last block of rows and of columns."""
+    n = k = 65536
+    w = torch.empty((n, k), dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator().manual_seed(10)
+    some = (torch.randn((256, k), generator=g) * k ** -0.5).to(torch.bfloat16)
+    w.view(-1, 256, k).copy_(some.to(DEV).expand(n // 256, 256, k))
+    w[-128:] *= -2
+    q, s = fp8.quantize_weight(w)
+    last = w[-128:].cpu()
+    cols = w[:, -128:].contiguous().cpu()
+    del w
+    rq, rb = R.quant(last, 128)
+    assert torch.equal(q[-128:].cpu().to(torch.float32).to(D), rq) and torch.equal(s[-1:].cpu().view(torch.uint8).to(torch.int64), rb)
+    wl, wc = R.deq(last, 128), R.deq(cols, 128)
+    for S in (3, 70):
+        x, dy = _rows(g, S, k, torch.bfloat16), _rows(g, S, n, torch.bfloat16, 0.1)
+        xg = x.to(DEV).requires_grad_(True)
+        y = fp8.linear(xg, q, s)
+        ref, tol = R.product(R.deq(x), wl)
+        R.check16(y[:, -128:], ref, tol, "last columns")
+        dx, = torch.autograd.grad(y, xg, dy.to(DEV))
+        ref, tol = R.product(R.deq(dy), wc.t().contiguous())
+        R.check16(dx[:, -128:], ref, tol, "last columns of the gradient")

@@ -253,3 +253,28 @@ def test_gradients_of_both_inputs_are_their_own():
         s.add_(1)
     with pytest.raises(RuntimeError):
         y.float().sum().backward()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 elements: every copy of the same 1024 rows gets the same result, forward, 8-bit output and backward."""
+    S, M, P = 2 ** 21 + 5, 2064, 1024
+    x, r, w = (t.to(DEV) for t in _data(P, M, torch.bfloat16, 7))
+    big_x, big_r = (t.repeat(S // P + 1, 1)[:S] for t in (x, r))
+
+    def same(t, u):
+        assert torch.equal(t[:S // P * P].view((S // P, P) + t.shape[1:]), u.expand((S // P,) + u.shape))
+        assert torch.equal(t[S // P * P:], u[:S % P])
+
+    with torch.no_grad():
+        rows, y, s = norm.add_rms_norm_fp8(big_x, big_r, w)
+        # 4096 rows and more take the one-wave form: the copies are compared with its own first rows
+        for t in (rows.q.view(torch.uint8), rows.scale.view(torch.uint8), y, s):
+            same(t, t[:P].clone())
+        small = norm.add_rms_norm_fp8(x, r, w)
+        assert torch.equal(s[:P], small[2])
+        R.check16(y[-P:], small[1].roll(-(S % P), 0).cpu().to(D), 2.0 ** -7 * small[1].roll(-(S % P), 0).cpu().to(D).abs(), "y")
+        del rows, y, s, big_r
+    xg = big_x.requires_grad_(True)
+    y = norm.rms_norm(xg, w)
+    dx, = torch.autograd.grad(y, xg, big_x.detach())
+    same(dx, dx[:P].clone())
