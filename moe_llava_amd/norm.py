@@ -53,8 +53,9 @@ def _as(t: Tensor, x: Tensor) -> Tensor:
 def _launch(x: Tensor, r: Optional[Tensor], w: Tensor, code: int, eps: float, want_y: bool, want_q: bool, want_rstd: bool):
     S, M = x.shape
     dev = x.device
-    y = torch.empty((S, M), dtype=x.dtype, device=dev) if want_y else None
-    s = torch.empty((S, M), dtype=x.dtype, device=dev) if r is not None else None
+    new = torch.empty_like if x.is_contiguous() else lambda t: torch.empty((S, M), dtype=t.dtype, device=dev)   # 1.2 us, 1.7
+    y = new(x) if want_y else None
+    s = new(x) if r is not None else None
     rstd = torch.empty((S,), dtype=torch.float32, device=dev) if want_rstd else None
     rows = _empty_rows(S, M, dev) if want_q else None
     if S:
