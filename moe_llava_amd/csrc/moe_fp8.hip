@@ -31,7 +31,8 @@
 // accumulators and v_maximum3 for the block maxima: gelu_new 27424 x 2560 x 10240 x 2 1364 -> 1325 us, SwiGLU -1 %).
 // Tried without gain: persistent blocks that start the next tile under the epilogue (49 spilled registers; 45056 rows 1.40 ->
 // 1.52 ms, 1408 rows 94 -> 106 us for the MLP), an epilogue instance per bias and mask (116 and more spilled registers),
-// super-rows of 2 to 16 row tiles (within 2 %, 16: -7 %), 8-bit outputs stored to stay in the caches (0.3 %), a deeper ring for the 32-row tiles, other read-ahead depths.
+// super-rows of 2 to 16 row tiles (within 2 %, 16: -7 %), 8-bit outputs stored to stay in the caches (0.3 %), 32 x 32 x 64
+// fragments for the 256 x 256 tile (plain products 3 % slower, the MLPs 1 %), a deeper ring for the 32-row tiles, other read-ahead depths.
 #include "moe_fp8.h"
 
 namespace moe {

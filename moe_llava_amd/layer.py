@@ -67,6 +67,7 @@ class MoE(nn.Module):
         if on and self.ep_size > 1:
             raise NotImplementedError("8-bit experts run on one GPU (ep_size == 1)")
         self.deepspeed_moe.experts.quantize_fp8(on)
+        self.deepspeed_moe.__dict__.pop("_decode_plans", None)       # they hold the other form's weights
         return self
 
     def forward_normed(self, hidden_states: Tensor, residual: Optional[Tensor], norm: nn.Module, used_token: Optional[Tensor] = None):
