@@ -43,10 +43,11 @@ def _blocks(n: int) -> int:
 
 
 def _empty_rows(S: int, K: int, dev) -> Fp8Rows:
-    kb = _blocks(K)
+    kb = (K + BLOCK - 1) // BLOCK
     q = torch.empty((S, K), dtype=E4M3, device=dev)
-    sc = torch.empty((S, (kb + 3) // 4 * 4), dtype=E8M0, device=dev)
-    return Fp8Rows(q, sc[:, :kb] if kb % 4 else sc)
+    if not kb % 4:
+        return Fp8Rows(q, torch.empty((S, kb), dtype=E8M0, device=dev))
+    return Fp8Rows(q, torch.empty((S, (kb + 3) // 4 * 4), dtype=E8M0, device=dev)[:, :kb])
 
 
 #: pointer of the current stream of a device, by index (torch.cuda.current_stream builds a Stream object per call: 1.9 us
@@ -133,7 +134,8 @@ def _check_weight(w: Tensor, ws: Tensor, name: str, E: int, N: Optional[int], pa
     n //= parts
     if K % 16 or not 16 <= K <= MAX_K:
         raise ValueError(f"{name}: K={K} must be a multiple of 16 and at most {MAX_K}")
-    if sc[-2] != parts * _blocks(n) or sc[-1] != _blocks(K) or (E and (sh[0] != E or sc[0] != E)) or ws.device != w.device:
+    if sc[-2] != parts * ((n + 127) // BLOCK) or sc[-1] != (K + 127) // BLOCK or (E and (sh[0] != E or sc[0] != E)) \
+            or ws.device != w.device:
         raise ValueError(f"{name}_scale: {tuple(sc)} on {ws.device} does not match {name} {tuple(sh)} on {w.device}")
     if w.data_ptr() % 16:
         raise ValueError(f"{name}: must be 16-byte aligned")

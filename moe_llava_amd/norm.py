@@ -31,16 +31,16 @@ def _weight_code(w: Tensor, x: Tensor) -> int:
 def _check(x: Tensor, residual: Optional[Tensor], weight: Tensor):
     x2 = _half_rows(x, "x")
     _gpu(weight, "weight")
-    M = x2.shape[1]
+    M, dev = x2.shape[1], x2.device
     if not 1 <= M <= MAX_M:
         raise ValueError(f"x: row length {M} must be between 1 and {MAX_M}")
-    if tuple(weight.shape) != (M,) or weight.device != x2.device:
-        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} does not match x {tuple(x.shape)} on {x2.device}")
+    if weight.dim() != 1 or weight.shape[0] != M or weight.device != dev:
+        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} does not match x {tuple(x.shape)} on {dev}")
     if not weight.is_contiguous():
         weight = weight.contiguous()
     r2 = None
     if residual is not None:
-        if not isinstance(residual, Tensor) or residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+        if not isinstance(residual, Tensor) or residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
             raise ValueError("residual must match x in shape, type and device")
         r2 = _half_rows(residual, "residual")
     return x2, r2, weight, _weight_code(weight, x2)
@@ -58,14 +58,19 @@ def _launch(x: Tensor, r: Optional[Tensor], w: Tensor, code: int, eps: float, wa
     s = new(x) if r is not None else None
     rstd = torch.empty((S,), dtype=torch.float32, device=dev) if want_rstd else None
     rows = _empty_rows(S, M, dev) if want_q else None
-    if S:
-        with ops._on(dev):
-            rc = _lib.load().moe_add_rms_norm_fwd(
-                x.data_ptr(), _lead(x, M), r.data_ptr() if r is not None else None, _lead(r, M) if r is not None else 0,
-                w.data_ptr(), code, eps, S, M, y.data_ptr() if want_y else None, M, s.data_ptr() if s is not None else None,
-                M, rstd.data_ptr() if want_rstd else None, rows.q.data_ptr() if want_q else None, M,
-                rows.scale.data_ptr() if want_q else None, _lead_scale(rows.scale) if want_q else 0, ops._dt(x),
-                _stream(dev.index))
+    if not S:
+        return y, s, rstd, rows
+    rp = ldr = sp = qp = qs = ldq = None
+    if r is not None:
+        rp, ldr, sp = r.data_ptr(), _lead(r, M), s.data_ptr()
+    if want_q:
+        q, sc = rows
+        qp, qs, ldq = q.data_ptr(), sc.data_ptr(), _lead_scale(sc)
+    with ops._on(dev):
+        rc = _lib.load().moe_add_rms_norm_fwd(
+            x.data_ptr(), _lead(x, M), rp, ldr or 0, w.data_ptr(), code, eps, S, M, y.data_ptr() if want_y else None, M, sp, M,
+            rstd.data_ptr() if want_rstd else None, qp, M, qs, ldq or 0, ops._dt(x), _stream(dev.index))
+    if rc:
         _lib.check(rc, "moe_add_rms_norm_fwd")
     return y, s, rstd, rows
 
