@@ -23,16 +23,20 @@
 // where fp32 products of the same 8-bit operands give 0.0017 (bf16's own rounding) and 0.0002.  The format's own noise is
 // 0.026.  The bf16 instruction on converted operands would be exact at half the rate; the rate is what 8-bit experts are for.
 //
-// Bound and measured.  Long products: the matrix pipe behind the LDS fills and the clock.  The 256 x 256 tile fills 64 KiB a
-// slice, 1.15 us at the 13 TB/s that the caches deliver to 256 CUs together; the fixed part of a tile (first fills, scales,
-// epilogue: 5 to 6.5 us) is hidden by nothing, as one block fills a CU's LDS.  8192 x 8192 x 8192: 2.77 PFLOP/s.
+// Bound and measured.  A slice of the 256 x 256 tile takes 1.39 us when every fill hits a cache (a timing copy that re-reads two
+// slices) and 1.45 to 1.65 with the fills from memory; its matrix instructions take 1.05 at the 1.95 GHz that the card holds
+// under them, and so do its LDS accesses (192 KiB read, 64 KiB filled).  So 12 % at 45056 x 5632 x 2048 and 3 % at 8192^3 is what
+// the memory side still costs.  The fixed part of a tile (first fills, scales, epilogue: 5 to 6.5 us) is hidden by nothing, as
+// one block fills a CU's LDS.  8192 x 8192 x 8192: 2.77 PFLOP/s.
 // 22528 x 2048 x 5632 (K 2048: 16 slices a tile): 247 us = 2.10 PFLOP/s; 45056 x 5632 x 2048: 467-490 us = 2.1-2.2; the gated
 // product of 45056 x 2048 x 11264: 0.93-1.11 ms = 1.9-2.2 (its epilogue is 3 to 4 us of vector work a tile; bias in the
 // accumulators and v_maximum3 for the block maxima: gelu_new 27424 x 2560 x 10240 x 2 1364 -> 1325 us, SwiGLU -1 %).
 // Tried without gain: persistent blocks that start the next tile under the epilogue (49 spilled registers; 45056 rows 1.40 ->
 // 1.52 ms, 1408 rows 94 -> 106 us for the MLP), an epilogue instance per bias and mask (116 and more spilled registers),
 // super-rows of 2 to 16 row tiles (within 2 %, 16: -7 %), 8-bit outputs stored to stay in the caches (0.3 %), 32 x 32 x 64
-// fragments for the 256 x 256 tile (plain products 3 % slower, the MLPs 1 %), a deeper ring for the 32-row tiles, other read-ahead depths.
+// fragments for the 256 x 256 tile (plain products 3 % slower, the MLPs 1 %), the same in slices of 64 columns and a ring of four
+// (12 % slower), fills issued between the matrix instructions (2 to 5 % slower), weight and row fragments read in other orders
+// (1 %), a deeper ring for the 32-row tiles, other read-ahead depths.
 #include "moe_fp8.h"
 
 namespace moe {
