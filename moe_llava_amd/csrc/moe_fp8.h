@@ -74,7 +74,7 @@ struct Fp8GemmParams {
     int K, N_out;
     int b_row_offset;         // gated: weight row of the first 'b' projection row (= N_out)
     int b_blk_offset;         // gated: row of the scales' grid where the 'b' projection starts
-    int n_gated;
+    int n_gated;              // gated: columns from here on are not gated; < N_out, or INT_MAX (all are gated)
     int col_tiles, rs;
     int vec_store;            // 16-bit output: rows and pointer allow 16-byte stores
     int zero_tail;            // 16-bit output: rows of [0, max_rows) that belong to no group are set to 0

@@ -39,6 +39,8 @@
 // (1 %), a deeper ring for the 32-row tiles, other read-ahead depths.
 #include "moe_fp8.h"
 
+#include <climits>
+
 namespace moe {
 
 constexpr int FTHREADS = 512;
@@ -394,8 +396,9 @@ __global__ __launch_bounds__(FTHREADS, 2) void fp8_gemm_kernel(const Fp8GemmPara
             }
         } else {
             // activation in fp32, the maximum of every row's block of 128 columns over the four lanes of a row (shuffles) and
-            // over the waves of the block (LDS), then e4m3 into the image.  Columns behind N_out repeat the last real one:
-            // they belong to the same block, so its maximum is not changed, and they are not stored.
+            // over the waves of the block (LDS), then e4m3 into the image.  Columns behind N_out repeat the last real one, its
+            // gate included (n_gated never lies between the two): they belong to the same block, so its maximum is not
+            // changed, and they are not stored.
             constexpr int GW = QB / CW;                        // waves that share a block of 128 columns
             unsigned *const top = reinterpret_cast<unsigned *>(lds + T::TOP);
             float mx[MFW];
@@ -814,7 +817,9 @@ extern "C" int moe_expert_ffn_fp8_fwd(int act, const void *x, int64_t ldx, int s
     p.group_offsets = group_offsets; p.G = G; p.n_experts = n_experts_local; p.max_rows = max_rows;
     p.out = ws.hq; p.ldo = I; p.out_scale = ws.hs; p.ld_os = ws.ld_hs;
     p.K = M; p.N_out = I; p.b_row_offset = I; p.b_blk_offset = ib;
-    p.n_gated = (n_gated < 0 || n_gated > I) ? I : n_gated;
+    // no mask: no column is past it.  The columns behind I that the last tile computes as repeats of column I - 1 count in a
+    // block's maximum, so they have to be gated as that column is (with a mask, n_gated < I: both lie behind it).
+    p.n_gated = (n_gated < 0 || n_gated >= I) ? INT_MAX : n_gated;
     if ((rc = fp8_gemm(p, gated ? MOE_EPI_SWIGLU : MOE_EPI_GELU_NEW, dtype, (hipStream_t)stream))) return rc;
     p = plain_params(ws.hq, I, ws.hs, ws.ld_hs, nullptr, 0, w2, w2_scale, b2, group_offsets, G, n_experts_local, max_rows, I, M, 0, y, M);
     p.splitk_ws = ws.split;
