@@ -217,17 +217,20 @@ class Experts(nn.Module):
             warnings.warn("moe_llava_amd.Experts: expert parameters are views into a buffer owned by someone else (a "
                           "flattening optimizer / engine); they are left where they are and copied into the packed "
                           "kernel layout on every forward (one pass over the expert weights per call)", stacklevel=3)
-        w1 = torch.zeros((E, nproj * Ip, M), **kw)
-        w2 = torch.zeros((E, M, Ip), **kw)
-        b1 = torch.zeros((E, nproj * Ip), **kw) if has_b1 else None
-        b2 = torch.zeros((E, M), **kw) if has_b2 else None
-        pk = {"w1": w1, "b1": b1, "w2": w2, "b2": b2}
-        self._copy_in(specs, pk)
-        if not external:
-            for lin, wv, bv in self._views(specs, pk):
-                lin.weight.data = wv
-                if bv is not None:
-                    lin.bias.data = bv
+        # normal tensors also when the first call runs in inference mode: a Parameter pointed at an inference tensor keeps a
+        # version that no longer moves, and cannot be trained afterwards
+        with torch.inference_mode(False), torch.no_grad():
+            w1 = torch.zeros((E, nproj * Ip, M), **kw)
+            w2 = torch.zeros((E, M, Ip), **kw)
+            b1 = torch.zeros((E, nproj * Ip), **kw) if has_b1 else None
+            b2 = torch.zeros((E, M), **kw) if has_b2 else None
+            pk = {"w1": w1, "b1": b1, "w2": w2, "b2": b2}
+            self._copy_in(specs, pk)
+            if not external:
+                for lin, wv, bv in self._views(specs, pk):
+                    lin.weight.data = wv
+                    if bv is not None:
+                        lin.bias.data = bv
         self._packed = pk
         self._external = external
         self._ptrs = [(p.data_ptr(), tuple(p.shape)) for p in self._params(specs)]
