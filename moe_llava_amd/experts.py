@@ -302,7 +302,8 @@ class Experts(nn.Module):
                                 or (old[3] is None) != (b1 is None) or (old[6] is None) != (b2 is None)
                                 or (old[3] is not None and old[3].dtype != b1.dtype)):
             old = None
-        with torch.no_grad():
+        # normal tensors whatever mode the first call runs in: a later refill may run in another
+        with torch.inference_mode(False), torch.no_grad():
             q1, s1 = fp8.quantize_weight(w1, nproj, out=old[1:3] if old else None)
             q2, s2 = fp8.quantize_weight(w2, out=old[4:6] if old else None)
             # biases stay in 16 bits; copies, like the weights, so that a call uses one state of them all

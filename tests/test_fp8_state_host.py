@@ -58,3 +58,20 @@ def test_packing_in_inference_mode_leaves_trainable_parameters():
         assert not p.is_inference()
         p.float().square().sum().backward()
         assert p.grad is not None
+
+
+@pytest.mark.parametrize("first", [torch.inference_mode, torch.no_grad])
+@pytest.mark.parametrize("then", [torch.inference_mode, torch.no_grad])
+def test_refill_in_another_mode(made, first, then):
+    """The copy made in one mode is filled again in the other, biases included, and stays the same tensors."""
+    ex = _experts(PhiMLP)
+    with first():
+        a = ex.packed_fp8(CPU)
+    with torch.no_grad():
+        for e in ex.deepspeed_experts:
+            e.fc1.weight.mul_(2)
+            e.fc2.bias.fill_(3)
+    with then():
+        b = ex.packed_fp8(CPU)
+    assert b is a and len(made) == 4 and all(bool((t == 3).all()) for t in b[6])
+    assert not any(t.is_inference() for t in b[1:] if t is not None)
