@@ -127,8 +127,15 @@ class Experts(nn.Module):
         self.n_gated: int = -1
         #: the experts run in 8 bits (``quantize_fp8``); the 16-bit parameters stay as they are
         self.fp8: bool = False
-        self._fp8 = None                      # (device, parameter versions, tensors, parameter addresses)
+        self._fp8 = None                      # (device, parameter versions, tensors, parameter addresses, ops.StreamOrder)
         self._register_state_dict_hook(_contiguous_state_dict)
+
+    def __getstate__(self):
+        """A copy (copy.deepcopy, torch.save) makes its own 8-bit weights: events and streams belong to this process."""
+        state = self.__dict__.copy()
+        state["_fp8"] = None
+        state.pop("_fast", None)
+        return state
 
     # ---- packed weights ----------------------------------------------------------------------
     def _specs(self) -> List[ExpertSpec]:
@@ -283,10 +290,12 @@ class Experts(nn.Module):
 
     def packed_fp8(self, device: torch.device):
         """(act, w1, w1_scale, b1|None, w2, w2_scale, b2|None) of the 8-bit experts, quantised from ``packed()``.  When the
-        16-bit weights change, the same tensors are filled again: a captured graph that reads them stays valid."""
+        16-bit weights change, the same tensors are filled again: a captured graph that reads them stays valid.  The current
+        stream is behind the filling when this returns, whichever stream that ran on."""
         cur = self._fp8
         if cur is not None and cur[0] == device and cur[1] is not None and self.packed_unchanged() is not None \
                 and cur[1] == self._versions([c[2] for c in self._fast[0]]):
+            cur[4].read()
             return cur[2]
         from . import fp8
         act, w1, b1, w2, b2 = self.packed(device)
@@ -295,6 +304,7 @@ class Experts(nn.Module):
         self._remember_fast(specs, (act, w1, b1, w2, b2))
         versions = self._versions(params)
         if cur is not None and cur[0] == device and versions is not None and cur[1] == versions and cur[3] == self._ptrs and not self._external:
+            cur[4].read()
             return cur[2]
         nproj = len(specs[0].fc1)
         old = cur[2] if cur is not None and cur[0] == device else None
@@ -302,6 +312,8 @@ class Experts(nn.Module):
                                 or (old[3] is None) != (b1 is None) or (old[6] is None) != (b2 is None)
                                 or (old[3] is not None and old[3].dtype != b1.dtype)):
             old = None
+        if old is not None:
+            cur[4].rewrite()
         # normal tensors whatever mode the first call runs in: a later refill may run in another
         with torch.inference_mode(False), torch.no_grad():
             q1, s1 = fp8.quantize_weight(w1, nproj, out=old[1:3] if old else None)
@@ -310,7 +322,9 @@ class Experts(nn.Module):
             c1, c2 = (old[3].copy_(b1) if b1 is not None else None, old[6].copy_(b2) if b2 is not None else None) if old \
                 else (b1.clone() if b1 is not None else None, b2.clone() if b2 is not None else None)
         out = old if old else (act, q1, s1, c1, q2, s2, c2)
-        self._fp8 = (device, versions, out, self._ptrs)
+        order = cur[4] if old else ops.StreamOrder(device, out[1:])
+        order.wrote()
+        self._fp8 = (device, versions, out, self._ptrs, order)
         return out
 
     def _views(self, specs, pk):

@@ -124,6 +124,61 @@ def _on(dev: torch.device):
     return torch.cuda.device(dev)
 
 
+def _stream_key(dev: torch.device):
+    """What tells the current stream of ``dev`` from others (None on the CPU, which has none)."""
+    if dev.type != "cuda":
+        return None
+    return torch._C._cuda_getCurrentRawStream(dev.index if dev.index is not None else torch.cuda.current_device())
+
+
+def _torch_stream(dev: torch.device):
+    return torch.cuda.current_stream(dev) if dev.type == "cuda" else None
+
+
+def _capturing(dev: torch.device) -> bool:
+    """Whether the current stream is being captured into a graph."""
+    return dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
+class StreamOrder:
+    """Order between the kernels that fill tensors which a module makes by itself and the calls that read them on whatever
+    stream they run: the user, who does not see the filling, cannot order it.  ``wrote`` behind the filling; ``read`` in front
+    of every use (a dict lookup once a stream has waited for the filling); ``rewrite`` in front of filling the same tensors
+    again.  A capture records no wait: what was filled before it began is waited for by ``torch.cuda.graph`` itself, and its
+    replays run on streams that are not known here."""
+    __slots__ = ("dev", "tensors", "done", "streams")
+
+    def __init__(self, dev: torch.device, tensors):
+        self.dev, self.tensors = dev, [t for t in tensors if t is not None]
+        self.done = None
+        self.streams = {}                     # streams that are behind the last filling
+
+    def wrote(self) -> None:
+        st = _torch_stream(self.dev)
+        self.done = st.record_event() if st is not None else None
+        self.streams = {}
+        self._seen(st)
+
+    def read(self) -> None:
+        if _stream_key(self.dev) in self.streams or _capturing(self.dev):
+            return
+        st = _torch_stream(self.dev)
+        st.wait_event(self.done)
+        self._seen(st)
+
+    def rewrite(self) -> None:
+        st, key = _torch_stream(self.dev), _stream_key(self.dev)
+        for k, other in self.streams.items():
+            if k != key:
+                st.wait_stream(other)
+
+    def _seen(self, st) -> None:
+        self.streams[_stream_key(self.dev)] = st
+        for t in self.tensors:
+            if t.is_cuda:
+                t.record_stream(st)           # freed memory is not handed out again before this stream is done with it
+
+
 _SPLITK_WS = {}      # (device index, stream pointer) -> 64 MiB workspace of the split-K tail
 _SPLITK_BYTES = None
 

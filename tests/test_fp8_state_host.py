@@ -1,10 +1,13 @@
 """The state that 8-bit experts keep between calls (the packed 16-bit weights, the 8-bit copy of them), on the CPU: the
 quantisation itself is replaced by a stand-in that records what it was asked to do."""
+import copy
+import pickle
+
 import pytest
 import torch
 
 import moe_llava_amd
-from moe_llava_amd import fp8
+from moe_llava_amd import fp8, ops
 from tests.expert_mlps import PhiMLP, StableLMMLP
 
 CPU = torch.device("cpu")
@@ -75,3 +78,84 @@ def test_refill_in_another_mode(made, first, then):
         b = ex.packed_fp8(CPU)
     assert b is a and len(made) == 4 and all(bool((t == 3).all()) for t in b[6])
     assert not any(t.is_inference() for t in b[1:] if t is not None)
+
+
+class _Stream:
+    """Stand-in of a stream: what was launched on it, in order, with the waits between."""
+    def __init__(self, log, name):
+        self.log, self.name, self.past = log, name, set()
+
+    def run(self, what):
+        self.past.add(what)
+        self.log.append((self.name, what))
+
+    def record_event(self):
+        return frozenset(self.past)
+
+    def wait_event(self, past):
+        self.past |= past
+
+    def wait_stream(self, other):
+        self.past |= other.past
+
+
+@pytest.fixture
+def streams(monkeypatch, made):
+    """Three streams of a pretended device; ``use(i)`` makes one current, fillings are launched on the current one."""
+    st = [_Stream([], i) for i in range(3)]
+    now = [0]
+    monkeypatch.setattr(ops, "_stream_key", lambda dev: now[0])
+    monkeypatch.setattr(ops, "_torch_stream", lambda dev: st[now[0]])
+    fill = fp8.quantize_weight
+
+    def quantize_weight(w, projections=1, out=None):
+        res = fill(w, projections, out)
+        st[now[0]].run(("fill", len(made)))
+        return res
+
+    monkeypatch.setattr(fp8, "quantize_weight", quantize_weight)
+
+    def use(i):
+        now[0] = i
+        return st[i]
+
+    return use
+
+
+def test_another_stream_is_behind_the_first_filling(streams, made):
+    ex = _experts()
+    streams(0)
+    ex.packed_fp8(CPU)
+    for i in (1, 2, 1, 0):
+        s = streams(i)
+        ex.packed_fp8(CPU)
+        assert {("fill", 1), ("fill", 2)} <= s.past and len(made) == 2
+
+
+def test_refilling_is_ordered_both_ways(streams, made):
+    """A refill runs behind what other streams launched before it, and in front of what they launch after it."""
+    ex = _experts()
+    streams(0)
+    ex.packed_fp8(CPU)
+    s1 = streams(1)
+    ex.packed_fp8(CPU)
+    s1.run("product")
+    with torch.no_grad():
+        ex.deepspeed_experts[0].up_proj.weight.mul_(2)
+    s2 = streams(2)
+    ex.packed_fp8(CPU)
+    assert "product" in s2.past and len(made) == 4
+    for i in (0, 1):
+        s = streams(i)
+        ex.packed_fp8(CPU)
+        assert {("fill", 3), ("fill", 4)} <= s.past and len(made) == 4
+
+
+def test_a_copy_of_the_module_makes_its_own(made):
+    ex = _experts()
+    a = ex.packed_fp8(CPU)
+    ex._fp8[4].done = lambda: None                       # stands for an event, which no copy can hold
+    for other in (copy.deepcopy(ex), pickle.loads(pickle.dumps(ex))):
+        assert other.fp8 and other._fp8 is None and ex._fp8[2] is a
+        b = other.packed_fp8(CPU)
+        assert b is not a and torch.equal(b[1], a[1])
