@@ -48,7 +48,8 @@ class GraphedMoE:
         if seed is None:
             seed = int(torch.randint(1, 2 ** 62, (1,), dtype=torch.int64).item())
         self.seed_dev = torch.tensor([seed], dtype=torch.int64, device=dev)
-        self.x = example.detach().clone()
+        with torch.inference_mode(False):      # a normal tensor: calls may come in another mode than this one
+            self.x = example.detach().clone()
         self.graph = torch.cuda.CUDAGraph()
         gate.__dict__["noise_seed_dev"] = self.seed_dev
         # a decode step's buffers belong to its plan; the captured step gets plans of its own, or two graphs of one layer
@@ -91,6 +92,6 @@ class GraphedMoE:
         if fp8 is not self._fp8 or n_gated != self._n_gated:
             raise ValueError("GraphedMoE: captured on another form of the experts (16-bit, another 8-bit copy, or another "
                              "number of gated channels): capture again")
-        self.x.copy_(x)
+        self.x.copy_(x.detach())               # gradients are not recorded
         self.graph.replay()
         return self.out

@@ -1,0 +1,75 @@
+"""What 8-bit experts keep between calls, on the GPU: streams, modes, graphs."""
+import pytest
+import torch
+
+import moe_llava_amd
+from moe_llava_amd import ops
+from moe_llava_amd.graph import GraphedMoE
+from tests.test_gpu_fp8_block import _moe, _x
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("S", [8, 300])
+@pytest.mark.parametrize("form", ["swiglu", "gelu_new"])
+def test_first_call_and_refill_seen_from_two_streams(S, form):
+    """No call before the streams part: the second stream's call is behind the filling that the first one launched."""
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    x = _x(S, 1024)
+    want = _moe(M=1024, I=2048, form=form).quantize_experts()
+    moe = _moe(M=1024, I=2048, form=form).quantize_experts()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        for _ in range(3):
+            ref = want(x)[0].clone()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(a):
+                y = moe(x)[0]
+            with torch.cuda.stream(b):
+                z = moe(x)[0]
+            torch.cuda.synchronize()
+            assert torch.equal(y, ref) and torch.equal(z, ref)
+            for m in (want, moe):
+                for p in m.deepspeed_moe.experts.parameters():
+                    p.mul_(0.5)
+            torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("S", [8, 100])
+@pytest.mark.parametrize("form", ["swiglu", "gelu_new"])
+def test_modes_mixed(S, form):
+    """First call in inference mode, weights changed in it and outside, calls and replays in either mode."""
+    moe, want = _moe(form=form).quantize_experts(), _moe(form=form).quantize_experts()
+    x = _x(S, 256)
+    with torch.inference_mode():
+        assert torch.equal(moe(x)[0], want(x)[0])
+        g = GraphedMoE(moe, x)
+        for m in (moe, want):
+            for p in m.deepspeed_moe.experts.parameters():
+                p.mul_(2)
+        assert torch.equal(moe(x)[0], want(x)[0]) and torch.equal(g(x)[0], want(x)[0])
+    with torch.no_grad():
+        for m in (moe, want):
+            for p in m.deepspeed_moe.experts.parameters():
+                p.mul_(0.5)
+        ref = want(x)[0].clone()
+        assert torch.equal(moe(x)[0], ref) and torch.equal(g(x)[0], ref)
+    for p in moe.deepspeed_moe.experts.parameters():
+        assert not p.is_inference()
+
+
+def test_graphed_step_takes_inputs_of_any_mode():
+    """Captured in inference mode, called outside it and with an input that requires a gradient (none is recorded)."""
+    for eight in (False, True):
+        moe = _moe()
+        if eight:
+            moe.quantize_experts()
+        x = _x(8, 256)
+        with torch.inference_mode():
+            g = GraphedMoE(moe, x)
+        with torch.no_grad():
+            ref = moe(x)[0].clone()
+        for _ in range(3):
+            out = g(x.clone().requires_grad_(True))[0]
+            assert torch.equal(out, ref) and not out.requires_grad and g.x.grad_fn is None
