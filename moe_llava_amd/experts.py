@@ -121,6 +121,7 @@ class Experts(nn.Module):
                 p.group_name = expert_group_name
         self._packed: Optional[Dict[str, Optional[Tensor]]] = None
         self._ptrs: Optional[List[int]] = None
+        self._order: Optional[ops.StreamOrder] = None      # of the packed buffers
         #: the parameters live in somebody else's flat buffer: never re-pointed, copied into the packed layout per forward
         self._external: bool = False
         #: SwiGLU channels >= n_gated skip the SiLU (RePaMLP experts); -1 = ordinary experts.  Refreshed per forward.
@@ -133,7 +134,7 @@ class Experts(nn.Module):
     def __getstate__(self):
         """A copy (copy.deepcopy, torch.save) makes its own 8-bit weights: events and streams belong to this process."""
         state = self.__dict__.copy()
-        state["_fp8"] = None
+        state["_fp8"] = state["_order"] = None
         state.pop("_fast", None)
         return state
 
@@ -169,12 +170,15 @@ class Experts(nn.Module):
         return ps
 
     def packed(self, device: torch.device):
-        """Return (act, w1 [E,N1,M], b1|None, w2 [E,M,I], b2|None), (re)packing when a parameter's storage moved."""
+        """Return (act, w1 [E,N1,M], b1|None, w2 [E,M,I], b2|None), (re)packing when a parameter's storage moved.  The current
+        stream is behind the packing when this returns, whichever stream that ran on."""
         specs = self._specs()
         params = self._params(specs)
         ptrs = [(p.data_ptr(), tuple(p.shape)) for p in params]   # reparam() keeps the address and shrinks the shape
         if self._packed is not None and ptrs == self._ptrs and self._packed["w1"].device == device:
             pk = self._packed
+            if self._order is not None:
+                self._order.read()
             if self._external:
                 self._copy_in(specs, pk)
             return specs[0].act, pk["w1"], pk["b1"], pk["w2"], pk["b2"]
@@ -241,6 +245,8 @@ class Experts(nn.Module):
         self._packed = pk
         self._external = external
         self._ptrs = [(p.data_ptr(), tuple(p.shape)) for p in self._params(specs)]
+        self._order = ops.StreamOrder(device, pk.values())
+        self._order.wrote()
         return specs[0].act, w1, b1, w2, b2
 
     def packed_unchanged(self):
@@ -255,6 +261,8 @@ class Experts(nn.Module):
             if d.get(name) is not prm or prm.data_ptr() != ptr or prm.shape[0] != n0:
                 self.__dict__["_fast"] = None
                 return None
+        if self._order is not None:
+            self._order.read()
         return fast[1]
 
     def _remember_fast(self, specs, result) -> None:

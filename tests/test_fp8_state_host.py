@@ -159,3 +159,17 @@ def test_a_copy_of_the_module_makes_its_own(made):
         assert other.fp8 and other._fp8 is None and ex._fp8[2] is a
         b = other.packed_fp8(CPU)
         assert b is not a and torch.equal(b[1], a[1])
+
+
+@pytest.mark.parametrize("again", ["packed", "packed_unchanged", "packed_fp8"])
+def test_another_stream_is_behind_the_packing(streams, monkeypatch, again):
+    ex = _experts(eight=again == "packed_fp8")
+    s0 = streams(0)
+    copy_in = ex._copy_in
+    monkeypatch.setattr(ex, "_copy_in", lambda *a: (copy_in(*a), s0.run("pack"))[0])
+    pk = ex.packed(CPU)
+    ex._remember_fast(ex._specs(), pk)
+    s1 = streams(1)
+    assert "pack" not in s1.past
+    getattr(ex, again)(*(() if again == "packed_unchanged" else (CPU,)))
+    assert "pack" in s1.past
