@@ -182,6 +182,10 @@ class Experts(nn.Module):
             if self._external:
                 self._copy_in(specs, pk)
             return specs[0].act, pk["w1"], pk["b1"], pk["w2"], pk["b2"]
+        if ops._capturing(device):
+            # the copies would run at the replays only, from parameters whose memory is free by then
+            raise RuntimeError("the first call of an MoE block packs its expert weights and cannot be captured: run it once "
+                               "before the capture")
         dtype = params[0].dtype
         for p in params:
             if p.dtype not in ops.HALF_DTYPES or p.dtype != dtype:
@@ -315,7 +319,10 @@ class Experts(nn.Module):
             cur[4].read()
             return cur[2]
         nproj = len(specs[0].fc1)
-        old = cur[2] if cur is not None and cur[0] == device else None
+        # in a capture the quantisation runs at the replays: into tensors of the graph's own, which follow the weights from then
+        # on, and never into the copy that calls outside the graph read
+        capturing = ops._capturing(device)
+        old = cur[2] if cur is not None and cur[0] == device and not capturing else None
         if old is not None and (old[0] != act or old[1].shape != w1.shape or old[4].shape != w2.shape
                                 or (old[3] is None) != (b1 is None) or (old[6] is None) != (b2 is None)
                                 or (old[3] is not None and old[3].dtype != b1.dtype)):
@@ -330,6 +337,8 @@ class Experts(nn.Module):
             c1, c2 = (old[3].copy_(b1) if b1 is not None else None, old[6].copy_(b2) if b2 is not None else None) if old \
                 else (b1.clone() if b1 is not None else None, b2.clone() if b2 is not None else None)
         out = old if old else (act, q1, s1, c1, q2, s2, c2)
+        if capturing:
+            return out
         order = cur[4] if old else ops.StreamOrder(device, out[1:])
         order.wrote()
         self._fp8 = (device, versions, out, self._ptrs, order)

@@ -173,3 +173,30 @@ def test_another_stream_is_behind_the_packing(streams, monkeypatch, again):
     assert "pack" not in s1.past
     getattr(ex, again)(*(() if again == "packed_unchanged" else (CPU,)))
     assert "pack" in s1.past
+
+
+def test_a_capture_leaves_the_copy_alone(monkeypatch, made):
+    """Quantised in a capture (no copy yet, or a stale one): tensors of the graph's own, never what other calls read."""
+    ex = _experts()
+    capture = lambda on: monkeypatch.setattr(ops, "_capturing", lambda dev: on)
+    capture(True)
+    with pytest.raises(RuntimeError, match="capture"):
+        ex.packed(CPU)
+    with pytest.raises(RuntimeError, match="capture"):
+        ex.packed_fp8(CPU)
+    capture(False)
+    ex.packed(CPU)
+    capture(True)
+    a = ex.packed_fp8(CPU)
+    assert ex._fp8 is None and len(made) == 2
+    capture(False)
+    b = ex.packed_fp8(CPU)
+    assert b is not a and len(made) == 4
+    capture(True)
+    assert ex.packed_fp8(CPU) is b and len(made) == 4                        # up to date: the graph reads the copy
+    with torch.no_grad():
+        ex.deepspeed_experts[1].down_proj.weight.mul_(2)
+    c = ex.packed_fp8(CPU)
+    assert c is not b and all(out is None for _, out in made[4:])
+    capture(False)
+    assert ex.packed_fp8(CPU) is b and len(made) == 8

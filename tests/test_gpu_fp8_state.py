@@ -73,3 +73,41 @@ def test_graphed_step_takes_inputs_of_any_mode():
         for _ in range(3):
             out = g(x.clone().requires_grad_(True))[0]
             assert torch.equal(out, ref) and not out.requires_grad and g.x.grad_fn is None
+
+
+def _capture(fn):
+    g = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(g):
+        out = fn()
+    return g, out
+
+
+@pytest.mark.parametrize("S", [8, 100])
+def test_capture_without_an_eager_call_in_8_bits(S):
+    """16-bit calls, then 8-bit experts whose first call is captured: eager calls before and between the replays are right,
+    and the graph, which quantises at every replay, follows the weights."""
+    moe, want = _moe(form="gelu_new"), _moe(form="gelu_new").quantize_experts()
+    x = _x(S, 256)
+    with torch.no_grad():
+        moe(x)
+        moe.quantize_experts()
+        g, (out, _, _) = _capture(lambda: moe(x))
+        for k in range(3):
+            ref = want(x)[0].clone()
+            assert torch.equal(moe(x)[0], ref)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, ref) and torch.equal(moe(x)[0], ref)
+            for m in (moe, want):
+                for p in m.deepspeed_moe.experts.parameters():
+                    p.mul_(0.5)
+
+
+def test_first_call_is_not_captured():
+    moe, x = _moe(), _x(8, 256)
+    g = torch.cuda.CUDAGraph()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(g):
+            moe(x)
+    with torch.no_grad():
+        assert torch.equal(moe(x)[0], _moe()(x)[0])                          # the module is as it was
