@@ -52,8 +52,7 @@ class GraphedMoE:
             self.x = example.detach().clone()
         self.graph = torch.cuda.CUDAGraph()
         gate.__dict__["noise_seed_dev"] = self.seed_dev
-        # a decode step's buffers belong to its plan; the captured step gets plans of its own, or two graphs of one layer
-        # (captured on the same stream) would write the same buffers when they are replayed on two streams
+        # the warm-up's plans live on a stream that nothing uses again: they go with it (the captured step has one of its own)
         plans = layer.__dict__.pop("_decode_plans", None)
         try:
             with torch.no_grad():
@@ -67,7 +66,7 @@ class GraphedMoE:
                     self.out = self._forward()
         finally:
             gate.__dict__.pop("noise_seed_dev", None)
-            self._plans = layer.__dict__.pop("_decode_plans", None)
+            layer.__dict__.pop("_decode_plans", None)
             if plans is not None:
                 layer.__dict__["_decode_plans"] = plans
         # 8-bit experts: the graph reads this copy of them; the reference keeps it alive, __call__ keeps it up to date

@@ -136,8 +136,11 @@ def _torch_stream(dev: torch.device):
 
 
 def _capturing(dev: torch.device) -> bool:
-    """Whether the current stream is being captured into a graph."""
-    return dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
+    """Whether the current stream of ``dev`` is being captured into a graph."""
+    if dev.type != "cuda":
+        return False
+    with _on(dev):
+        return torch.cuda.is_current_stream_capturing()
 
 
 class StreamOrder:

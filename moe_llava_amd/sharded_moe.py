@@ -162,7 +162,7 @@ class _DecodePlan:
 
     The buffers are REUSED: ``l_aux``, ``exp_counts``, ``gate.last_logits`` and ``last_routing`` of such a call are views
     that the module's next decode-size call overwrites (clone what must survive a later call); the output is a
-    fresh tensor every time."""
+    fresh tensor every time.  A step captured into a graph has a plan of its own that is not kept here."""
 
     __slots__ = ("args", "ref", "routing", "logits", "hy", "packed", "S", "M", "cap", "sampling", "fn", "l_aux", "exp_counts",
                  "dtype", "dev", "q", "qref")
@@ -513,7 +513,9 @@ class MOELayer(nn.Module):
             if experts.__dict__.get("_fast") is None:
                 return None                  # RePaMLP masks / externally owned parameters: the general path
         plans = d.get("_decode_plans")
-        if plans is None:
+        if ops._capturing(x.device):
+            plans = {}                       # a graph's step gets buffers of its own, from the graph's memory
+        elif plans is None:
             plans = d["_decode_plans"] = {}
         wgw = gate.wg.weight
         key = (experts.fp8, S, x.dtype, x.device.index, st, gate.training, wgw.data_ptr(), wgw.dtype, gate.capacity_factor,

@@ -200,3 +200,35 @@ def test_a_capture_leaves_the_copy_alone(monkeypatch, made):
     assert c is not b and all(out is None for _, out in made[4:])
     capture(False)
     assert ex.packed_fp8(CPU) is b and len(made) == 8
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_captured_decode_steps_keep_no_plan(monkeypatch, made, eight):
+    """Every captured step gets a plan (the step's buffers) of its own; steps outside a capture share theirs."""
+    from moe_llava_amd import sharded_moe
+    plans = []
+
+    class Plan:
+        def __init__(self, layer, x, packed, st):
+            self.packed, self.logits, self.exp_counts, self.routing, self.l_aux = packed, None, None, None, None
+            plans.append(self)
+
+        def run(self, gate, x, rows8=None):
+            self.ran = True
+            return x
+
+    monkeypatch.setattr(sharded_moe, "_DecodePlan", Plan)
+    monkeypatch.setattr(ops, "_stream_ptr", lambda t: 5)
+    moe = moe_llava_amd.MoE(64, StableLMMLP(64, 64).to(torch.bfloat16), num_experts=2, k=2)
+    layer = moe.quantize_experts(eight).deepspeed_moe
+    x = torch.zeros((1, 64), dtype=torch.bfloat16)
+    step = lambda: layer._decode_step(x, x, 1)
+    step(), step()
+    assert len(plans) == 1
+    monkeypatch.setattr(ops, "_capturing", lambda dev: True)
+    step(), step()
+    assert len(plans) == 3 and all(p.ran for p in plans)
+    assert list(layer.__dict__["_decode_plans"].values()) == plans[:1]
+    monkeypatch.setattr(ops, "_capturing", lambda dev: False)
+    step()
+    assert len(plans) == 3

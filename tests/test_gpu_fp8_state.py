@@ -111,3 +111,27 @@ def test_first_call_is_not_captured():
             moe(x)
     with torch.no_grad():
         assert torch.equal(moe(x)[0], _moe()(x)[0])                          # the module is as it was
+
+
+@pytest.mark.parametrize("S", [8, 100])
+@pytest.mark.parametrize("eight", [False, True])
+def test_two_graphs_captured_by_hand(S, eight):
+    """Two steps of one layer captured on one stream: neither writes what the other returned, and eager calls (here of enough
+    different sizes that the kept plans are dropped) leave both alone."""
+    moe = _moe()
+    if eight:
+        moe.quantize_experts()
+    a, b = _x(S, 256, seed=5), _x(S, 256, seed=6)
+    with torch.no_grad():
+        ra, rb = [t.clone() for t in moe(a)], [t.clone() for t in moe(b)]
+        (g1, o1), (g2, o2) = _capture(lambda: moe(a)), _capture(lambda: moe(b))
+        for _ in range(3):
+            g1.replay(), g2.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(o1, ra)) and all(torch.equal(p, q) for p, q in zip(o2, rb))
+            g2.replay()
+            for s in range(1, 40):
+                moe(a[:s])
+            g1.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(o1, ra)) and all(torch.equal(p, q) for p, q in zip(o2, rb))
