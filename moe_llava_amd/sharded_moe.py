@@ -254,10 +254,8 @@ class _DecodePlan:
                 q.xq, q.ld_xq, q.xq_scale, q.ld_xs = fp8.row_pointers(rows8, self.S, self.M, self.dev)
             else:
                 q.xq, q.ld_xq, q.xq_scale, q.ld_xs = None, 0, None, 0
-            with ops._on(self.dev):
-                rc = self.fn(self.ref, self.qref)
-        else:
-            rc = self.fn(self.ref)
+        with ops._on(self.dev):
+            rc = self.fn(self.ref) if self.q is None else self.fn(self.ref, self.qref)
         if rc:
             from . import _lib
             _lib.check(rc, "moe_block_top2_fp8_fwd" if self.q is not None else "moe_block_top2_fwd_args")

@@ -232,3 +232,27 @@ def test_captured_decode_steps_keep_no_plan(monkeypatch, made, eight):
     monkeypatch.setattr(ops, "_capturing", lambda dev: False)
     step()
     assert len(plans) == 3
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_decode_step_runs_on_its_device(monkeypatch, eight):
+    """The library launches on the current device, which need not be the one that the tokens are on."""
+    import contextlib
+    from moe_llava_amd import _lib, sharded_moe
+    current, ran_on = ["other"], []
+
+    @contextlib.contextmanager
+    def on(dev):
+        current.append(dev)
+        yield
+        current.pop()
+
+    monkeypatch.setattr(ops, "_on", on)
+    plan = object.__new__(sharded_moe._DecodePlan)
+    plan.args, plan.ref, plan.qref = _lib.BlockTop2Args(), None, None
+    plan.q = _lib.Fp8Experts() if eight else None
+    plan.S, plan.M, plan.dtype, plan.dev, plan.sampling = 1, 64, torch.bfloat16, CPU, False
+    plan.fn = lambda *a: ran_on.append(current[-1]) or 0
+    gate = moe_llava_amd.TopKGate(64, 2, k=2)
+    plan.run(gate, torch.zeros((1, 64), dtype=torch.bfloat16))
+    assert ran_on == [CPU]
