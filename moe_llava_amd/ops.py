@@ -187,23 +187,28 @@ _SPLITK_BYTES = None
 
 
 def _splitk_ws(t: Tensor, st: int):
-    """(pointer, bytes) of the split-K workspace of the grouped GEMM launches on stream ``st`` of ``t``'s device
+    """(pointer, bytes, owner) of the split-K workspace of the grouped GEMM launches on stream ``st`` of ``t``'s device
     (include/moe_gfx950.h: moe_splitk_workspace_bytes).  One buffer per (device, stream), allocated on first use and kept:
     launches on one stream are ordered, launches on different streams (the chunks of the expert-parallel exchange
-    alternate between two) must not share it.  ``MOE_SPLITK=0`` in the environment: no workspace, tiles stay whole."""
+    alternate between two) must not share it.  Launches that are captured get one from the graph's memory, as graphs
+    captured on one stream may be replayed on several; the caller holds ``owner`` until its launches are out.
+    ``MOE_SPLITK=0`` in the environment: no workspace, tiles stay whole."""
     global _SPLITK_BYTES
     if _SPLITK_BYTES is None:
         import os
         env = os.environ.get("MOE_SPLITK")
         _SPLITK_BYTES = 0 if (env is not None and int(env) < 2) else int(_lib.load().moe_splitk_workspace_bytes())
     if _SPLITK_BYTES == 0 or not t.is_cuda:
-        return None, 0
+        return None, 0, None
+    if _capturing(t.device):
+        ws = torch.empty((_SPLITK_BYTES,), dtype=torch.uint8, device=t.device)
+        return ws.data_ptr(), _SPLITK_BYTES, ws
     key = (t.device.index, st)
     ws = _SPLITK_WS.get(key)
     if ws is None:
         ws = torch.empty((_SPLITK_BYTES,), dtype=torch.uint8, device=t.device)
         _SPLITK_WS[key] = ws
-    return ws.data_ptr(), _SPLITK_BYTES
+    return ws.data_ptr(), _SPLITK_BYTES, ws
 
 
 def reload_knobs() -> None:
@@ -443,7 +448,7 @@ def _expert_ffn_launch(act, a, gather_ptr, gather_shift, w1, b1, w2, b2, offs_pt
     b1p = b1.data_ptr() if b1 is not None else None
     b2p = b2.data_ptr() if b2 is not None else None
     st = _stream_ptr(a)
-    skp, skb = _splitk_ws(a, st)
+    skp, skb, sk_owner = _splitk_ws(a, st)
     with _on(dev):
         if timer is None:
             rc = lib.moe_expert_ffn_fwd(act, a.data_ptr(), a.stride(0), gather_ptr, gather_shift, w1.data_ptr(), b1p,
@@ -530,7 +535,7 @@ def block_top2(x: Tensor, wg_weight: Tensor, capacity: int, noise: Optional[Tens
     out = torch.empty((S, M), dtype=x.dtype, device=dev)
     hp = hy.data_ptr()
     st = _stream_ptr(x)
-    skp, skb = _splitk_ws(x, st) if max_rows > 64 else (None, 0)     # decode-size launches take the GEMV-style kernel
+    skp, skb, sk_owner = _splitk_ws(x, st) if max_rows > 64 else (None, 0, None)     # decode-size launches take the GEMV-style kernel
     if noise_seed_dev is not None:
         _need(noise_seed_dev, "noise_seed_dev", torch.int64)
         if noise is not None or noise_seed_dev.numel() != 1 or noise_seed_dev.device != dev:
@@ -661,7 +666,7 @@ def expert_ffn_train(act: int, a: Tensor, gather: Optional[Tensor], gather_shift
         return y, ab, h
     lib = _lib.load()
     st = _stream_ptr(a)
-    skp, skb = _splitk_ws(a, st)
+    skp, skb, sk_owner = _splitk_ws(a, st)
     with _on(dev):
         rc = lib.moe_expert_ffn_fwd_train(
             act, a.data_ptr(), a.stride(0), gather.data_ptr() if gather is not None else None, gather_shift,

@@ -256,3 +256,16 @@ def test_a_decode_step_runs_on_its_device(monkeypatch, eight):
     gate = moe_llava_amd.TopKGate(64, 2, k=2)
     plan.run(gate, torch.zeros((1, 64), dtype=torch.bfloat16))
     assert ran_on == [CPU]
+
+
+def test_captured_launches_share_no_splitk_workspace(monkeypatch):
+    from types import SimpleNamespace
+    monkeypatch.setattr(ops, "_SPLITK_BYTES", 4096)
+    monkeypatch.setattr(ops, "_SPLITK_WS", {})
+    t = SimpleNamespace(is_cuda=True, device=CPU)
+    eager = ops._splitk_ws(t, 7)
+    assert ops._splitk_ws(t, 7)[0] == eager[0] != ops._splitk_ws(t, 8)[0]
+    monkeypatch.setattr(ops, "_capturing", lambda dev: True)
+    held = [ops._splitk_ws(t, 7) for _ in range(2)]
+    assert len({eager[0], held[0][0], held[1][0]}) == 3 and all(h[2].data_ptr() == h[0] for h in held)
+    assert len(ops._SPLITK_WS) == 2

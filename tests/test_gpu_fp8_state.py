@@ -135,3 +135,20 @@ def test_two_graphs_captured_by_hand(S, eight):
             g1.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(o1, ra)) and all(torch.equal(p, q) for p, q in zip(o2, rb))
+
+
+def test_two_captured_steps_of_16_bit_experts_on_two_streams():
+    """Sizes whose products cut their last round along K: each graph has a workspace of its own."""
+    moe = _moe(M=1024, I=4096)
+    a, b = _x(1500, 1024, seed=5), _x(1500, 1024, seed=6)
+    with torch.no_grad():
+        ra, rb = moe(a)[0].clone(), moe(b)[0].clone()
+        (g1, o1), (g2, o2) = _capture(lambda: moe(a)), _capture(lambda: moe(b))
+        st = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s, g in zip(st, (g1, g2)):
+                with torch.cuda.stream(s):
+                    g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o1[0], ra) and torch.equal(o2[0], rb)
