@@ -75,8 +75,8 @@ class MoE(nn.Module):
         ``residual`` None, ``hidden_states``),
         ``forward(rms_norm(s))``.  Returns ``(output, l_aux, exp_counts, s)``; the layer's output is ``s + output``.  ``norm``:
         a root-mean-square norm with ``weight`` and ``eps`` (or ``variance_epsilon``).  With 8-bit experts the norm's launch
-        writes the rows in 8 bits beside the 16-bit rows that the gate reads, otherwise, and for a subclass with a ``forward``
-        of its own or a module with hooks, this is ``norm.add_rms_norm`` and ``forward``."""
+        writes the rows in 8 bits beside the 16-bit rows that the gate reads, otherwise, and where this module or its
+        ``deepspeed_moe`` has hooks or a ``forward`` of its own, this is ``norm.add_rms_norm`` and ``forward``."""
         from . import norm as norm_ops
         from .sharded_moe import module_has_hooks
         if isinstance(norm, nn.LayerNorm) or getattr(norm, "bias", None) is not None:
@@ -85,8 +85,8 @@ class MoE(nn.Module):
         if eps is None:
             eps = norm.variance_epsilon
         layer = self.deepspeed_moe
-        if not self.use_residual and type(self).forward is MoE.forward and not module_has_hooks(self) \
-                and layer.takes_fp8_rows(hidden_states, used_token):
+        plain = lambda m, cls: type(m).forward is cls.forward and "forward" not in m.__dict__ and not module_has_hooks(m)
+        if not self.use_residual and plain(self, MoE) and plain(layer, MOELayer) and layer.takes_fp8_rows(hidden_states, used_token):
             rows, y, s = norm_ops.add_rms_norm_fp8(hidden_states, residual, norm.weight, eps)
             out = layer(y, used_token, rows)
             return out, layer.l_aux, layer.exp_counts, s

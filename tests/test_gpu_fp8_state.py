@@ -2,8 +2,7 @@
 import pytest
 import torch
 
-import moe_llava_amd
-from moe_llava_amd import ops
+from moe_llava_amd import norm
 from moe_llava_amd.graph import GraphedMoE
 from tests.test_gpu_fp8_block import _moe, _x
 
@@ -152,3 +151,22 @@ def test_two_captured_steps_of_16_bit_experts_on_two_streams():
                     g.replay()
             torch.cuda.synchronize()
             assert torch.equal(o1[0], ra) and torch.equal(o2[0], rb)
+
+
+@pytest.mark.parametrize("S", [8, 100])
+def test_normed_block_keeps_what_is_around_the_inner_layer(S):
+    """A hook on, or a forward of, the layer inside the module may change what the experts get: the rows that the norm's launch
+    wrote in 8 bits are not theirs then."""
+    moe = _moe().quantize_experts()
+    nm = norm.RMSNorm(256, eps=1e-5, dtype=torch.bfloat16, device=DEV)
+    x, r = _x(S, 256, seed=3), _x(S, 256, seed=4)
+    layer = moe.deepspeed_moe
+    with torch.no_grad():
+        y = norm.add_rms_norm(x, r, nm.weight, 1e-5)[0]
+        want = moe(y * 2)[0].clone()
+        h = layer.register_forward_pre_hook(lambda m, args: (args[0] * 2,) + args[1:])
+        assert torch.equal(moe.forward_normed(x, r, nm)[0], want)
+        h.remove()
+        inner = layer.forward
+        layer.forward = lambda a, used_token=None: inner(a * 2, used_token)
+        assert torch.equal(moe.forward_normed(x, r, nm)[0], want)
