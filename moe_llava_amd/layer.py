@@ -73,27 +73,30 @@ class MoE(nn.Module):
     def forward_normed(self, hidden_states: Tensor, residual: Optional[Tensor], norm: nn.Module, used_token: Optional[Tensor] = None):
         """The step of a pre-norm decoder layer in front of and through the block: ``s = hidden_states + residual`` (or, with
         ``residual`` None, ``hidden_states``),
-        ``forward(rms_norm(s))``.  Returns ``(output, l_aux, exp_counts, s)``; the layer's output is ``s + output``.  ``norm``:
-        a root-mean-square norm with ``weight`` and ``eps`` (or ``variance_epsilon``).  With 8-bit experts the norm's launch
-        writes the rows in 8 bits beside the 16-bit rows that the gate reads, otherwise, and where this module or its
+        ``forward(norm(s))``.  Returns ``(output, l_aux, exp_counts, s)``; the layer's output is ``s + output``.  ``norm``: a
+        root-mean-square norm; ``norm.RMSNorm``, ``torch.nn.RMSNorm`` with an eps, and classes given to
+        ``norm.register_rms_norm`` run as kernels, any other (and one with hooks) is called.  With 8-bit experts the norm's
+        launch writes the rows in 8 bits beside the 16-bit rows that the gate reads, otherwise, and where this module or its
         ``deepspeed_moe`` has hooks or a ``forward`` of its own, this is ``norm.add_rms_norm`` and ``forward``."""
         from . import norm as norm_ops
         from .sharded_moe import module_has_hooks
         if isinstance(norm, nn.LayerNorm) or getattr(norm, "bias", None) is not None:
             raise TypeError(f"forward_normed: {type(norm).__name__} is no root-mean-square norm with a weight only")
-        eps = getattr(norm, "eps", None)
-        if eps is None:
-            eps = norm.variance_epsilon
+        known = norm_ops.weight_and_eps(norm)
+        if known is None:
+            s = hidden_states if residual is None else hidden_states + residual
+            return (*self(norm(s), used_token), s)
+        weight, eps = known
         layer = self.deepspeed_moe
         plain = lambda m, cls: type(m).forward is cls.forward and "forward" not in m.__dict__ and not module_has_hooks(m)
         if not self.use_residual and plain(self, MoE) and plain(layer, MOELayer) and layer.takes_fp8_rows(hidden_states, used_token):
-            rows, y, s = norm_ops.add_rms_norm_fp8(hidden_states, residual, norm.weight, eps)
+            rows, y, s = norm_ops.add_rms_norm_fp8(hidden_states, residual, weight, eps)
             out = layer(y, used_token, rows)
             return out, layer.l_aux, layer.exp_counts, s
         if residual is None:
-            y, s = norm_ops.rms_norm(hidden_states, norm.weight, eps), hidden_states
+            y, s = norm_ops.rms_norm(hidden_states, weight, eps), hidden_states
         else:
-            y, s = norm_ops.add_rms_norm(hidden_states, residual, norm.weight, eps)
+            y, s = norm_ops.add_rms_norm(hidden_states, residual, weight, eps)
         out, l_aux, exp_counts = self(y, used_token)
         return out, l_aux, exp_counts, s
 

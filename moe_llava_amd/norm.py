@@ -19,6 +19,8 @@ from .fp8 import Fp8Rows, _empty_rows, _gpu, _half_rows, _lead, _lead_scale, _st
 
 MAX_M = 65536
 
+_FORWARDS = {nn.RMSNorm.forward}     # forwards that are ``rms_norm(x, self.weight, self.eps)``
+
 
 def _weight_code(w: Tensor, x: Tensor) -> int:
     if w.dtype == torch.float32:
@@ -149,6 +151,29 @@ def add_rms_norm_fp8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps:
     return rows, (_as(y, x) if want_y else None), (_as(s, x) if s is not None else x)
 
 
+def register_rms_norm(cls):
+    """Declare that ``cls.forward(x)`` is ``rms_norm(x, self.weight, self.eps)`` (or ``self.variance_epsilon``), up to the
+    roundings in between, so that ``MoE.forward_normed`` may run the kernel in its place.  Returns ``cls``."""
+    _FORWARDS.add(cls.forward)
+    return cls
+
+
+def weight_and_eps(module: nn.Module):
+    """(weight, eps) of a norm module whose call is known to be ``rms_norm`` of them, else None: a forward that is not declared
+    (it may scale by 1 + weight), hooks, no weight, or an eps that the module leaves to torch."""
+    from .sharded_moe import module_has_hooks
+    if type(module).forward not in _FORWARDS or "forward" in module.__dict__ or module_has_hooks(module):
+        return None
+    weight = getattr(module, "weight", None)
+    eps = getattr(module, "eps", None)
+    if eps is None:
+        eps = getattr(module, "variance_epsilon", None)
+    if not isinstance(weight, Tensor) or weight.dim() != 1 or eps is None:
+        return None
+    return weight, eps
+
+
+@register_rms_norm
 class RMSNorm(nn.Module):
     """``weight`` and ``eps`` of a root-mean-square norm (the attribute names of the reference's RMSNorm modules are
     ``weight`` and ``eps`` / ``variance_epsilon``); ``forward(x)`` or ``forward(x, residual)`` -> y or (y, s)."""

@@ -170,3 +170,27 @@ def test_normed_block_keeps_what_is_around_the_inner_layer(S):
         inner = layer.forward
         layer.forward = lambda a, used_token=None: inner(a * 2, used_token)
         assert torch.equal(moe.forward_normed(x, r, nm)[0], want)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_norms_in_front_of_the_block(eight):
+    """torch's own norm with an eps runs as the kernel; without one, and a norm that scales by 1 + weight, as they are."""
+    class OnePlus(torch.nn.RMSNorm):
+        def forward(self, x):
+            return (x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + 1e-5) * (1 + self.weight.float())).to(x.dtype)
+
+    moe = _moe()
+    if eight:
+        moe.quantize_experts()
+    x, r = _x(20, 256, seed=3), _x(20, 256, seed=4)
+    mk = dict(dtype=torch.bfloat16, device=DEV)
+    with torch.no_grad():
+        w = (1 + 0.1 * torch.randn(256)).to(torch.bfloat16).to(DEV)
+        own, theirs = norm.RMSNorm(256, 1e-5, **mk), torch.nn.RMSNorm(256, 1e-5, **mk)
+        for nm in (own, theirs):
+            nm.weight.copy_(w)
+        a, b = moe.forward_normed(x, r, own), moe.forward_normed(x, r, theirs)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[3], b[3])
+        for nm in (torch.nn.RMSNorm(256, **mk), torch.nn.RMSNorm(256, elementwise_affine=False), OnePlus(256, **mk)):
+            out, la, ec, s = moe.forward_normed(x, r, nm)
+            assert torch.equal(s, x + r) and torch.equal(out, moe(nm(x + r))[0])
