@@ -342,6 +342,11 @@ class MOELayer(nn.Module):
         #: run the exchange path even when ep_size == 1 (single-rank group; exercises the RCCL code on one GPU)
         self.force_exchange: bool = False
 
+    def __getstate__(self):
+        """A copy (copy.deepcopy, torch.save) builds its own plans: they hold addresses and streams of this process."""
+        drop = ("_decode_plans", "_side_stream", "_ep_plan_cache")
+        return {k: v for k, v in self.__dict__.items() if k not in drop}
+
     def _set_ep_group(self, ep_group):
         self.ep_group = ep_group
         self.gate._set_ep_group(ep_group)

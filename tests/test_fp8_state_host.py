@@ -269,3 +269,13 @@ def test_captured_launches_share_no_splitk_workspace(monkeypatch):
     held = [ops._splitk_ws(t, 7) for _ in range(2)]
     assert len({eager[0], held[0][0], held[1][0]}) == 3 and all(h[2].data_ptr() == h[0] for h in held)
     assert len(ops._SPLITK_WS) == 2
+
+
+def test_a_copy_of_the_layer_has_no_plans():
+    from moe_llava_amd import _lib
+    moe = moe_llava_amd.MoE(64, StableLMMLP(64, 64).to(torch.bfloat16), num_experts=2, k=2)
+    plans = moe.deepspeed_moe.__dict__["_decode_plans"] = {0: _lib.BlockTop2Args()}
+    for other in (copy.deepcopy(moe), pickle.loads(pickle.dumps(moe))):
+        assert "_decode_plans" not in other.deepspeed_moe.__dict__
+        assert all(torch.equal(a, b) for a, b in zip(other.parameters(), moe.parameters()))
+    assert moe.deepspeed_moe._decode_plans is plans

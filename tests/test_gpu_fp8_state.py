@@ -194,3 +194,17 @@ def test_norms_in_front_of_the_block(eight):
         for nm in (torch.nn.RMSNorm(256, **mk), torch.nn.RMSNorm(256, elementwise_affine=False), OnePlus(256, **mk)):
             out, la, ec, s = moe.forward_normed(x, r, nm)
             assert torch.equal(s, x + r) and torch.equal(out, moe(nm(x + r))[0])
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_used_module_can_be_copied(eight):
+    import copy
+    moe, x = _moe(), _x(8, 256)
+    if eight:
+        moe.quantize_experts()
+    with torch.no_grad():
+        ref = moe(x)[0].clone()
+        other = copy.deepcopy(moe)
+        for p in other.deepspeed_moe.experts.parameters():
+            p.mul_(0.5)
+        assert torch.equal(moe(x)[0], ref) and not torch.equal(other(x)[0], ref)
