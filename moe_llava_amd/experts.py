@@ -14,6 +14,7 @@ the cheaper ``packed_unchanged()`` (identity and address of every parameter agai
 from __future__ import annotations
 
 import copy
+import threading
 from dataclasses import dataclass
 from typing import Callable, Dict, List, Optional
 
@@ -31,6 +32,9 @@ class ExpertSpec:
     fc2: nn.Linear
     n_gated: int = -1             # SWIGLU: hidden channels >= n_gated skip the SiLU (RePaMLP); -1 = all gated
 
+
+#: held while weights are packed or quantised: two threads whose first calls meet must not both re-point the parameters
+_FILLING = threading.RLock()
 
 _ADAPTERS: List[Callable[[nn.Module], Optional[ExpertSpec]]] = []
 
@@ -172,16 +176,30 @@ class Experts(nn.Module):
     def packed(self, device: torch.device):
         """Return (act, w1 [E,N1,M], b1|None, w2 [E,M,I], b2|None), (re)packing when a parameter's storage moved.  The current
         stream is behind the packing when this returns, whichever stream that ran on."""
+        res = self._packed_as_is(device)
+        if res is None:
+            with _FILLING:
+                res = self._packed_as_is(device) or self._pack(device)
+        return res
+
+    def _packed_as_is(self, device: torch.device):
         specs = self._specs()
         params = self._params(specs)
         ptrs = [(p.data_ptr(), tuple(p.shape)) for p in params]   # reparam() keeps the address and shrinks the shape
-        if self._packed is not None and ptrs == self._ptrs and self._packed["w1"].device == device:
-            pk = self._packed
-            if self._order is not None:
-                self._order.read()
-            if self._external:
-                self._copy_in(specs, pk)
-            return specs[0].act, pk["w1"], pk["b1"], pk["w2"], pk["b2"]
+        if self._packed is None or ptrs != self._ptrs:
+            return None
+        pk = self._packed
+        if pk["w1"].device != device:
+            return None
+        if self._order is not None:
+            self._order.read()
+        if self._external:
+            self._copy_in(specs, pk)
+        return specs[0].act, pk["w1"], pk["b1"], pk["w2"], pk["b2"]
+
+    def _pack(self, device: torch.device):
+        specs = self._specs()
+        params = self._params(specs)
         if ops._capturing(device):
             # the copies would run at the replays only, from parameters whose memory is free by then
             raise RuntimeError("the first call of an MoE block packs its expert weights and cannot be captured: run it once "
@@ -231,7 +249,7 @@ class Experts(nn.Module):
             import warnings
             warnings.warn("moe_llava_amd.Experts: expert parameters are views into a buffer owned by someone else (a "
                           "flattening optimizer / engine); they are left where they are and copied into the packed "
-                          "kernel layout on every forward (one pass over the expert weights per call)", stacklevel=3)
+                          "kernel layout on every forward (one pass over the expert weights per call)", stacklevel=4)
         # normal tensors also when the first call runs in inference mode: a Parameter pointed at an inference tensor keeps a
         # version that no longer moves, and cannot be trained afterwards
         with torch.inference_mode(False), torch.no_grad():
@@ -246,11 +264,10 @@ class Experts(nn.Module):
                     lin.weight.data = wv
                     if bv is not None:
                         lin.bias.data = bv
-        self._packed = pk
-        self._external = external
-        self._ptrs = [(p.data_ptr(), tuple(p.shape)) for p in self._params(specs)]
-        self._order = ops.StreamOrder(device, pk.values())
-        self._order.wrote()
+        order = ops.StreamOrder(device, pk.values())
+        order.wrote()
+        self._packed, self._external, self._order = pk, external, order
+        self._ptrs = [(p.data_ptr(), tuple(p.shape)) for p in self._params(specs)]      # last: what makes the others valid
         return specs[0].act, w1, b1, w2, b2
 
     def packed_unchanged(self):
@@ -304,12 +321,17 @@ class Experts(nn.Module):
         """(act, w1, w1_scale, b1|None, w2, w2_scale, b2|None) of the 8-bit experts, quantised from ``packed()``.  When the
         16-bit weights change, the same tensors are filled again: a captured graph that reads them stays valid.  The current
         stream is behind the filling when this returns, whichever stream that ran on."""
-        cur = self._fp8
-        if cur is not None and cur[0] == device and cur[1] is not None and self.packed_unchanged() is not None \
-                and cur[1] == self._versions([c[2] for c in self._fast[0]]):
+        cur, fast = self._fp8, self.__dict__.get("_fast")
+        if cur is not None and cur[0] == device and cur[1] is not None and fast is not None \
+                and self.packed_unchanged() is not None and cur[1] == self._versions([c[2] for c in fast[0]]):
             cur[4].read()
             return cur[2]
+        with _FILLING:
+            return self._fill_fp8(device)
+
+    def _fill_fp8(self, device: torch.device):
         from . import fp8
+        cur = self._fp8
         act, w1, b1, w2, b2 = self.packed(device)
         specs = self._specs()
         params = self._params(specs)

@@ -279,3 +279,35 @@ def test_a_copy_of_the_layer_has_no_plans():
         assert "_decode_plans" not in other.deepspeed_moe.__dict__
         assert all(torch.equal(a, b) for a, b in zip(other.parameters(), moe.parameters()))
     assert moe.deepspeed_moe._decode_plans is plans
+
+
+def _threads(n, fn):
+    """fn(i) in n threads at once; what they returned."""
+    import threading
+    out, go = [None] * n, threading.Barrier(n)
+
+    def run(i):
+        go.wait()
+        out[i] = fn(i)
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(n)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    return out
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_first_calls_of_several_threads(monkeypatch, made, eight):
+    """One packing and one quantisation, and parameters that all lie in the buffers that the calls got."""
+    import time
+    ex = _experts(eight=eight)
+    ref = [p.detach().clone() for p in ex.parameters()]
+    copy_in = ex._copy_in
+    monkeypatch.setattr(ex, "_copy_in", lambda *a: (time.sleep(0.05), copy_in(*a)))      # the threads meet in here
+    got = _threads(4, lambda i: ex.packed_fp8(CPU) if eight else ex.packed(CPU))
+    assert all(a is b for g in got for a, b in zip(g, got[0])) and len(made) == (2 if eight else 0)
+    own = {t.untyped_storage().data_ptr() for t in ex._packed.values() if t is not None}
+    assert all(p.untyped_storage().data_ptr() in own for p in ex.parameters())
+    assert all(torch.equal(a, b) for a, b in zip(ref, ex.parameters()))
