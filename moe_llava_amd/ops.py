@@ -5,6 +5,7 @@ Nothing here computes on the CPU or in eager torch; a missing library raises (``
 """
 from __future__ import annotations
 
+import threading
 from typing import Optional
 
 import torch
@@ -71,11 +72,15 @@ class PhaseTimer:
         return out
 
 
-_STREAM_SCOPE = None   # (device index, stream pointer) while MOELayer runs one forward; saves repeated lookups
+class _Scope(threading.local):
+    cur = None         # (device index, stream pointer) while MOELayer runs one forward in this thread; saves repeated lookups
+
+
+_SCOPE = _Scope()
 
 
 def _stream_ptr(t: Tensor) -> int:
-    sc = _STREAM_SCOPE
+    sc = _SCOPE.cur
     if sc is not None and sc[0] == t.device.index:
         return sc[1]
     return torch.cuda.current_stream(t.device).cuda_stream
@@ -89,15 +94,13 @@ class stream_scope:
         self.t = t
 
     def __enter__(self):
-        global _STREAM_SCOPE
-        self.prev = _STREAM_SCOPE
+        self.prev = _SCOPE.cur
         if self.t.is_cuda:
-            _STREAM_SCOPE = (self.t.device.index, torch.cuda.current_stream(self.t.device).cuda_stream)
+            _SCOPE.cur = (self.t.device.index, torch.cuda.current_stream(self.t.device).cuda_stream)
         return self
 
     def __exit__(self, *a):
-        global _STREAM_SCOPE
-        _STREAM_SCOPE = self.prev
+        _SCOPE.cur = self.prev
         return False
 
 
@@ -171,7 +174,7 @@ class StreamOrder:
 
     def rewrite(self) -> None:
         st, key = _torch_stream(self.dev), _stream_key(self.dev)
-        for k, other in self.streams.items():
+        for k, other in list(self.streams.items()):
             if k != key:
                 st.wait_stream(other)
 

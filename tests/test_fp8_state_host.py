@@ -311,3 +311,23 @@ def test_first_calls_of_several_threads(monkeypatch, made, eight):
     own = {t.untyped_storage().data_ptr() for t in ex._packed.values() if t is not None}
     assert all(p.untyped_storage().data_ptr() in own for p in ex.parameters())
     assert all(torch.equal(a, b) for a, b in zip(ref, ex.parameters()))
+
+
+def test_a_thread_keeps_its_stream(monkeypatch):
+    """The stream that a forward looks up once is that thread's, whatever other threads run meanwhile."""
+    import threading
+    from types import SimpleNamespace
+    mine = threading.local()
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: SimpleNamespace(cuda_stream=mine.stream))
+    t = SimpleNamespace(is_cuda=True, device=SimpleNamespace(index=0))
+    both = threading.Barrier(2)
+
+    def run(i):
+        mine.stream = 100 + i
+        with ops.stream_scope(t):
+            both.wait()
+            got = ops._stream_ptr(t)
+            both.wait()
+        return got
+
+    assert _threads(2, run) == [100, 101]
