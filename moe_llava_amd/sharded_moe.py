@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import math
 from typing import Optional
@@ -155,7 +156,7 @@ DECODE_MAX_TOKENS = 64      # calls of at most this many tokens take the cached 
 
 class _DecodePlan:
     """Everything one decode-size forward (S <= 64 tokens, one GPU, top-2, no grad) needs, built once per
-    (S, dtype, device, stream, training flag) and reused: the routing arena, logits and the h / y workspace, and the
+    (thread, S, dtype, device, stream, training flag) and reused: the routing arena, logits and the h / y workspace, and the
     argument block of ``moe_block_top2_fwd_args`` with every constant field filled in.  A call then rewrites three
     fields (x, the Gumbel seed, out) and makes ONE ctypes call with ONE argument: at S = 1 the kernels take ~45 us and
     the host side of the call was what bounded the step (profiles/r03/decode_host_*).
@@ -521,7 +522,7 @@ class MOELayer(nn.Module):
         elif plans is None:
             plans = d["_decode_plans"] = {}
         wgw = gate.wg.weight
-        key = (experts.fp8, S, x.dtype, x.device.index, st, gate.training, wgw.data_ptr(), wgw.dtype, gate.capacity_factor,
+        key = (threading.get_ident(), experts.fp8, S, x.dtype, x.device.index, st, gate.training, wgw.data_ptr(), wgw.dtype, gate.capacity_factor,
                gate.eval_capacity_factor, gate.min_capacity, gate.drop_tokens, gate.top2_2nd_expert_sampling, experts.n_gated)
         plan = plans.get(key)
         if plan is None or plan.packed is not packed:

@@ -331,3 +331,25 @@ def test_a_thread_keeps_its_stream(monkeypatch):
         return got
 
     assert _threads(2, run) == [100, 101]
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_threads_on_one_stream_have_plans_of_their_own(monkeypatch, made, eight):
+    from moe_llava_amd import sharded_moe
+
+    class Plan:
+        def __init__(self, layer, x, packed, st):
+            self.packed, self.logits, self.exp_counts, self.routing, self.l_aux = packed, None, None, None, None
+
+        def run(self, gate, x, rows8=None):
+            seen.append(self)
+            return x
+
+    seen = []
+    monkeypatch.setattr(sharded_moe, "_DecodePlan", Plan)
+    monkeypatch.setattr(ops, "_stream_ptr", lambda t: 5)
+    layer = moe_llava_amd.MoE(64, StableLMMLP(64, 64).to(torch.bfloat16), num_experts=2, k=2).quantize_experts(eight).deepspeed_moe
+    x = torch.zeros((1, 64), dtype=torch.bfloat16)
+    layer._decode_step(x, x, 1)
+    _threads(2, lambda i: (layer._decode_step(x, x, 1), layer._decode_step(x, x, 1)))
+    assert len(seen) == 5 and len(set(map(id, seen))) == 3
