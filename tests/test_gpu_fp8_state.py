@@ -208,3 +208,33 @@ def test_a_used_module_can_be_copied(eight):
         for p in other.deepspeed_moe.experts.parameters():
             p.mul_(0.5)
         assert torch.equal(moe(x)[0], ref) and not torch.equal(other(x)[0], ref)
+
+
+@pytest.mark.parametrize("S", [8, 200])
+@pytest.mark.parametrize("eight", [False, True])
+def test_threads_with_streams_of_their_own(S, eight):
+    """Four threads call one layer, first call included, each on its stream."""
+    import threading
+    ref, moe = _moe(), _moe()
+    if eight:
+        ref.quantize_experts(), moe.quantize_experts()
+    xs = [_x(S, 256, seed=20 + i) for i in range(4)]
+    with torch.no_grad():
+        want = [ref(x)[0].clone() for x in xs]
+    torch.cuda.synchronize()
+    got, go = [None] * 4, threading.Barrier(4)
+
+    def run(i):
+        st = torch.cuda.Stream()
+        go.wait()
+        with torch.no_grad(), torch.cuda.stream(st):
+            got[i] = [moe(xs[i])[0] for _ in range(20)]
+        st.synchronize()
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    for g, w in zip(got, want):
+        assert all(torch.equal(y, w) for y in g)
