@@ -270,11 +270,17 @@ class Experts(nn.Module):
         self._ptrs = [(p.data_ptr(), tuple(p.shape)) for p in self._params(specs)]      # last: what makes the others valid
         return specs[0].act, w1, b1, w2, b2
 
-    def packed_unchanged(self):
+    def packed_unchanged(self, stream=None):
         """The tuple ``packed()`` returned last time if nothing it depends on has moved since (same Parameter objects at
         the same addresses with the same leading size), else None -- the cheap check of the decode fast path, which
         is host-bound.  Experts whose parameters live in somebody else's buffer, or with a RePaMLP mask, always answer
-        None (they need the full ``packed()`` on every call)."""
+        None (they need the full ``packed()`` on every call).  ``stream``: the current stream's raw pointer, if known."""
+        res = self._unchanged()
+        if res is not None and self._order is not None:
+            self._order.read(stream)
+        return res
+
+    def _unchanged(self):
         fast = self.__dict__.get("_fast")
         if fast is None:
             return None
@@ -282,8 +288,6 @@ class Experts(nn.Module):
             if d.get(name) is not prm or prm.data_ptr() != ptr or prm.shape[0] != n0:
                 self.__dict__["_fast"] = None
                 return None
-        if self._order is not None:
-            self._order.read()
         return fast[1]
 
     def _remember_fast(self, specs, result) -> None:
@@ -317,14 +321,14 @@ class Experts(nn.Module):
         except RuntimeError:                  # parameters made in inference mode keep no version
             return None
 
-    def packed_fp8(self, device: torch.device):
+    def packed_fp8(self, device: torch.device, stream=None):
         """(act, w1, w1_scale, b1|None, w2, w2_scale, b2|None) of the 8-bit experts, quantised from ``packed()``.  When the
         16-bit weights change, the same tensors are filled again: a captured graph that reads them stays valid.  The current
-        stream is behind the filling when this returns, whichever stream that ran on."""
+        stream (``stream``: its raw pointer, if known) is behind the filling when this returns, whichever stream that ran on."""
         cur, fast = self._fp8, self.__dict__.get("_fast")
         if cur is not None and cur[0] == device and cur[1] is not None and fast is not None \
-                and self.packed_unchanged() is not None and cur[1] == self._versions([c[2] for c in fast[0]]):
-            cur[4].read()
+                and self._unchanged() is not None and cur[1] == self._versions([c[2] for c in fast[0]]):
+            cur[4].read(stream)
             return cur[2]
         with _FILLING:
             return self._fill_fp8(device)

@@ -14,8 +14,14 @@ import torch
 from torch import Tensor, nn
 from torch.nn import functional as F
 
+from . import norm as norm_ops
 from .experts import Experts
-from .sharded_moe import MOELayer, TopKGate
+from .sharded_moe import MOELayer, TopKGate, module_has_hooks
+
+
+def _as_written(m: nn.Module, cls) -> bool:
+    """Whether calling ``m`` runs ``cls.forward`` and nothing else."""
+    return type(m).forward is cls.forward and "forward" not in m.__dict__ and not module_has_hooks(m)
 
 
 class MoE(nn.Module):
@@ -78,18 +84,16 @@ class MoE(nn.Module):
         ``norm.register_rms_norm`` run as kernels, any other (and one with hooks) is called.  With 8-bit experts the norm's
         launch writes the rows in 8 bits beside the 16-bit rows that the gate reads, otherwise, and where this module or its
         ``deepspeed_moe`` has hooks or a ``forward`` of its own, this is ``norm.add_rms_norm`` and ``forward``."""
-        from . import norm as norm_ops
-        from .sharded_moe import module_has_hooks
-        if isinstance(norm, nn.LayerNorm) or getattr(norm, "bias", None) is not None:
-            raise TypeError(f"forward_normed: {type(norm).__name__} is no root-mean-square norm with a weight only")
         known = norm_ops.weight_and_eps(norm)
         if known is None:
+            if isinstance(norm, nn.LayerNorm) or getattr(norm, "bias", None) is not None:
+                raise TypeError(f"forward_normed: {type(norm).__name__} is no root-mean-square norm with a weight only")
             s = hidden_states if residual is None else hidden_states + residual
             return (*self(norm(s), used_token), s)
         weight, eps = known
-        layer = self.deepspeed_moe
-        plain = lambda m, cls: type(m).forward is cls.forward and "forward" not in m.__dict__ and not module_has_hooks(m)
-        if not self.use_residual and plain(self, MoE) and plain(layer, MOELayer) and layer.takes_fp8_rows(hidden_states, used_token):
+        layer = self._modules["deepspeed_moe"]
+        if not self.use_residual and _as_written(self, MoE) and _as_written(layer, MOELayer) \
+                and layer.takes_fp8_rows(hidden_states, used_token):
             rows, y, s = norm_ops.add_rms_norm_fp8(hidden_states, residual, weight, eps)
             out = layer(y, used_token, rows)
             return out, layer.l_aux, layer.exp_counts, s

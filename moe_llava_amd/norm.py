@@ -16,6 +16,7 @@ from torch import Tensor, nn
 
 from . import _lib, ops
 from .fp8 import Fp8Rows, _empty_rows, _gpu, _half_rows, _lead, _lead_scale, _stream
+from .sharded_moe import module_has_hooks
 
 MAX_M = 65536
 
@@ -161,11 +162,15 @@ def register_rms_norm(cls):
 def weight_and_eps(module: nn.Module):
     """(weight, eps) of a norm module whose call is known to be ``rms_norm`` of them, else None: a forward that is not declared
     (it may scale by 1 + weight), hooks, no weight, or an eps that the module leaves to torch."""
-    from .sharded_moe import module_has_hooks
-    if type(module).forward not in _FORWARDS or "forward" in module.__dict__ or module_has_hooks(module):
+    if getattr(type(module), "forward", None) not in _FORWARDS:
         return None
-    weight = getattr(module, "weight", None)
-    eps = getattr(module, "eps", None)
+    d = module.__dict__                       # plain dict access where it finds something: nn.Module.__getattr__ is slow
+    if "forward" in d or module_has_hooks(module):
+        return None
+    weight = d["_parameters"].get("weight")
+    if weight is None:
+        weight = getattr(module, "weight", None)
+    eps = d.get("eps")
     if eps is None:
         eps = getattr(module, "variance_epsilon", None)
     if not isinstance(weight, Tensor) or weight.dim() != 1 or eps is None:

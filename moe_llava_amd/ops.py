@@ -138,12 +138,17 @@ def _torch_stream(dev: torch.device):
     return torch.cuda.current_stream(dev) if dev.type == "cuda" else None
 
 
+_is_capturing = torch.cuda.is_current_stream_capturing
+
+
 def _capturing(dev: torch.device) -> bool:
     """Whether the current stream of ``dev`` is being captured into a graph."""
     if dev.type != "cuda":
         return False
-    with _on(dev):
-        return torch.cuda.is_current_stream_capturing()
+    if _current_device() == dev.index:
+        return _is_capturing()
+    with torch.cuda.device(dev):
+        return _is_capturing()
 
 
 class StreamOrder:
@@ -165,12 +170,14 @@ class StreamOrder:
         self.streams = {}
         self._seen(st)
 
-    def read(self) -> None:
-        if _stream_key(self.dev) in self.streams or _capturing(self.dev):
+    def read(self, key=None) -> None:
+        """``key``: the current stream's raw pointer, where the caller has it."""
+        if (_stream_key(self.dev) if key is None else key) in self.streams or _capturing(self.dev):
             return
         st = _torch_stream(self.dev)
-        st.wait_event(self.done)
-        self._seen(st)
+        if st is not None:
+            st.wait_event(self.done)
+            self._seen(st)
 
     def rewrite(self) -> None:
         st, key = _torch_stream(self.dev), _stream_key(self.dev)

@@ -14,6 +14,7 @@ from typing import Optional
 
 import numpy as np
 import torch
+import torch.nn.modules.module as _tm
 from torch import Tensor, nn
 
 from . import ops
@@ -165,8 +166,8 @@ class _DecodePlan:
     that the module's next decode-size call overwrites (clone what must survive a later call); the output is a
     fresh tensor every time.  A step captured into a graph has a plan of its own that is not kept here."""
 
-    __slots__ = ("args", "ref", "routing", "logits", "hy", "packed", "S", "M", "cap", "sampling", "fn", "l_aux", "exp_counts",
-                 "dtype", "dev", "q", "qref")
+    __slots__ = ("args", "refs", "routing", "logits", "hy", "packed", "S", "M", "cap", "sampling", "fn", "l_aux", "exp_counts",
+                 "dtype", "dev", "q")
 
     def __init__(self, layer: "MOELayer", x: Tensor, packed, st: int):
         """``packed``: ``Experts.packed()`` or, for 8-bit experts, ``Experts.packed_fp8()``."""
@@ -217,13 +218,12 @@ class _DecodePlan:
             q.w1, q.w1_scale, q.b1 = w1.data_ptr(), packed[2].data_ptr(), a.b1
             q.w2, q.w2_scale, q.b2 = w2.data_ptr(), packed[5].data_ptr(), a.b2
             q.workspace, q.ws_bytes = hp + yb, nws
-            self.qref = ctypes.byref(q)
         else:
             a.h_ws, a.y = hp, hp + rows * I * 2
             self.q = None
         a.splitk_ws, a.splitk_ws_bytes = None, 0         # decode-size launches take the GEMV-style kernel: nothing to split
         a.dtype, a.stream = ops._dt(x), st
-        self.args, self.ref = a, ctypes.byref(a)
+        self.args, self.refs = a, (ctypes.byref(a),) if self.q is None else (ctypes.byref(a), ctypes.byref(self.q))
         self.routing, self.packed, self.S, self.M, self.cap = r, packed, S, M, cap
         self.sampling = bool(gate.top2_2nd_expert_sampling)
         self.fn = lib.moe_block_top2_fp8_fwd if eight else lib.moe_block_top2_fwd_args
@@ -256,7 +256,7 @@ class _DecodePlan:
             else:
                 q.xq, q.ld_xq, q.xq_scale, q.ld_xs = None, 0, None, 0
         with ops._on(self.dev):
-            rc = self.fn(self.ref) if self.q is None else self.fn(self.ref, self.qref)
+            rc = self.fn(*self.refs)
         if rc:
             from . import _lib
             _lib.check(rc, "moe_block_top2_fp8_fwd" if self.q is not None else "moe_block_top2_fwd_args")
@@ -265,8 +265,8 @@ class _DecodePlan:
 
 def module_has_hooks(m: nn.Module) -> bool:
     """Any forward / forward-pre hook that nn.Module.__call__ would run for ``m`` (its own or torch's global ones)."""
-    import torch.nn.modules.module as tm
-    return bool(m._forward_hooks or m._forward_pre_hooks or tm._global_forward_hooks or tm._global_forward_pre_hooks)
+    d = m.__dict__                 # plain dict access: nn.Module.__getattr__ is slow on the decode path
+    return bool(d["_forward_hooks"] or d["_forward_pre_hooks"] or _tm._global_forward_hooks or _tm._global_forward_pre_hooks)
 
 
 def _fresh_seed() -> int:
@@ -509,7 +509,7 @@ class MOELayer(nn.Module):
         gate, experts = self.gate, self.experts
         d = self.__dict__
         st = ops._stream_ptr(x)
-        packed = experts.packed_fp8(x.device) if experts.fp8 else experts.packed_unchanged()
+        packed = experts.packed_fp8(x.device, st) if experts.fp8 else experts.packed_unchanged(st)
         if packed is None:
             packed = experts.packed(x.device)
             experts._remember_fast(experts._specs(), packed)

@@ -249,7 +249,7 @@ def test_a_decode_step_runs_on_its_device(monkeypatch, eight):
 
     monkeypatch.setattr(ops, "_on", on)
     plan = object.__new__(sharded_moe._DecodePlan)
-    plan.args, plan.ref, plan.qref = _lib.BlockTop2Args(), None, None
+    plan.args, plan.refs = _lib.BlockTop2Args(), (None,)
     plan.q = _lib.Fp8Experts() if eight else None
     plan.S, plan.M, plan.dtype, plan.dev, plan.sampling = 1, 64, torch.bfloat16, CPU, False
     plan.fn = lambda *a: ran_on.append(current[-1]) or 0
