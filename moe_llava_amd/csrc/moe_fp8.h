@@ -44,8 +44,11 @@ __device__ __forceinline__ unsigned umax_xor(unsigned v, int mask) {
     return v > o ? v : o;
 }
 
-// activations in fp32 (nothing is rounded between the accumulator and the quantisation: a 16-bit rounding there would move
-// ~1 % of the elements to a neighbouring e4m3 value)
+// Activations in fp32: nothing is rounded to 16 bits between the accumulator and the quantisation (that would move ~1 % of
+// the elements to a neighbouring e4m3 value).  v_exp_f32 and v_rcp_f32 are good to a unit in the last place each, and the
+// rounding of the exponential's argument t (a for silu, 2 u below) makes |t| 2^-23 of it: (|t| + 4) 2^-23 of the result, 2^-19
+// at |t| = 12, here and in fast_silu (moe_common.h).  The accumulators under them are good to 2^-16 (moe_fp8.hip), and e4m3's
+// half step is 2^-4.
 __device__ __forceinline__ float gelu_new_f32(float x) {
     // 0.5 x (1 + tanh u) = x / (1 + 2^(-2u log2 e)), u = sqrt(2 / pi) (x + 0.044715 x^3): the exponent is x (c0 + c1 x^2)
     constexpr float c0 = -2.f * 0.7978845608028654f * 1.4426950408889634f, c1 = c0 * 0.044715f;

@@ -567,6 +567,8 @@ static int launch_fp8_tile(Fp8GemmParams p, hipStream_t st) {
 // 10240, one group and four; microseconds).  The smallest estimate is within 5 % of the best of thirteen tiles on 39 of 44
 // swept shapes (100 ... 11264 rows, K 1024 ... 10240, N 1024 ... 5632, 1 to 8 groups), 1.6 % off on average and 21 % at worst;
 // the 256 x 256 tile alone is up to 3.2 x off there (1408 rows, K 5632, N 2048, 4 groups: 57.9 us against 30.9).
+// It ranks tiles; as a time it is low where a launch keeps all CUs busy for long and the clock falls: 4096 x 4096 x 10240 is
+// estimated at 110 us and takes 124 (1.39 us a slice, not 1.29), 11264 x 2560 -> 2048 in 8 groups at 62 and takes 68 to 80.
 // With a workspace, the 256 x 256 tile's last round may be cut along K (Fp8Sched): its estimate is then the whole rounds, a
 // piece of the tail, and the pieces written and read back (0.11 us each at 4.7 TB/s, 5 us for the launch).  6854 rows, K
 // 10240, N 2560 (290 tiles on 256 CUs): 264 us whole, 200 + 19 cut; pieces of 12, 20 or 26 slices the same, 40 slower.
