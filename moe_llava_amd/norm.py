@@ -172,6 +172,8 @@ def weight_and_eps(module: nn.Module):
         weight = getattr(module, "weight", None)
     eps = d.get("eps")
     if eps is None:
+        eps = getattr(module, "eps", None)
+    if eps is None:
         eps = getattr(module, "variance_epsilon", None)
     if not isinstance(weight, Tensor) or weight.dim() != 1 or eps is None:
         return None
