@@ -27,6 +27,14 @@ class _OnePlus(_Llama):
         return (1 + self.weight) * x * torch.rsqrt(x.square().mean(-1, keepdim=True) + self.variance_epsilon)
 
 
+class _Property(_Llama):
+    """An eps that is a property, and a forward of its own."""
+    eps = property(lambda self: 2e-5)
+
+    def forward(self, x):
+        return super().forward(x)
+
+
 @pytest.fixture
 def moe(monkeypatch):
     class Block(moe_llava_amd.MoE):
@@ -62,7 +70,8 @@ def test_other_norms_are_called(moe, make, res):
 
 
 @pytest.mark.parametrize("make,eps", [(lambda: norm_ops.RMSNorm(M, 1e-4), 1e-4), (lambda: nn.RMSNorm(M, 1e-3), 1e-3),
-                                      (lambda: norm_ops.register_rms_norm(_Llama)(), 1e-5)])
+                                      (lambda: norm_ops.register_rms_norm(_Llama)(), 1e-5),
+                                      (lambda: norm_ops.register_rms_norm(_Property)(), 2e-5)])
 @pytest.mark.parametrize("res", [False, True])
 def test_known_norms_run_as_kernels(moe, make, eps, res):
     nm = make()
