@@ -362,6 +362,7 @@ int moe_dispatch_bwd(const void *da_rows, const int32_t *expert_idx, const int32
  * max|block| * 2^-e <= 448 (scaling rounds nothing).  A block that holds an infinity or a NaN becomes NaN (byte 255), and so
  * does every product that reads it.  The last block of a row, and of a matrix in either direction, may be short.
  * Row scales: [rows, ceil(K/128)] with a row stride that is a multiple of 4 bytes, 4-byte aligned, the padding readable;
+ * rows (S, max_rows, src_rows) and matrix dimensions: at most 2^31 - 512.
  * weight scales: dense [experts, ceil(N/128), ceil(K/128)], for the gated W1 [experts, 2 * ceil(I/128), ceil(M/128)] (each
  * projection has a grid of its own). */
 

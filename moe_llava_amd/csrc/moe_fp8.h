@@ -17,6 +17,7 @@ typedef __attribute__((ext_vector_type(4))) int v4i_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 
 constexpr int QB = 128;               // elements that share a scale along K (and weight rows along N)
+constexpr int DIM_MAX = 0x7fffffff - 511;  // rows, and columns of either operand: rounding up to a tile (at most 256) stays in 32 bits
 inline bool grid_fits(long long blocks, int threads) { return blocks * threads <= 0xffffffffLL; }  // a launch has 2^32 - 1 threads at most
 constexpr unsigned E8M0_NAN = 255u;   // scale of a block that holds an infinity or a NaN; its elements are all NaN
 

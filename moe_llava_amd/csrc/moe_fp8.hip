@@ -674,6 +674,7 @@ static int fp8_args_ok(const char *fn, const void *a, int64_t lda, const void *a
     if (K < 16 || (K & 15) || K > FP8_MAX_K) return fail(MOE_ERR_SHAPE, "%s: need K %% 16 == 0, 16 <= K <= %d (K=%d)", fn, FP8_MAX_K, K);
     if (N < 1 || G < 1 || G > 4096 || n_experts < 1 || max_rows < 0 || gather_shift < 0 || gather_shift > 1)
         return fail(MOE_ERR_SHAPE, "%s: need N >= 1, 1 <= G <= 4096, experts >= 1, rows >= 0 (N=%d G=%d experts=%d rows=%d)", fn, N, G, n_experts, max_rows);
+    if (N > DIM_MAX || max_rows > DIM_MAX) return fail(MOE_ERR_SHAPE, "%s: N=%d, rows=%d: at most %d", fn, N, max_rows, DIM_MAX);
     if (lda < K || (lda & 15)) return fail(MOE_ERR_SHAPE, "%s: row stride %lld: need >= K and a multiple of 16", fn, (long long)lda);
     const int kb = (K + QB - 1) / QB;
     if (ld_as < kb || (ld_as & 3)) return fail(MOE_ERR_SHAPE, "%s: scale row stride %lld: need >= %d and a multiple of 4", fn, (long long)ld_as, kb);

@@ -403,7 +403,8 @@ extern "C" int moe_add_rms_norm_fwd(const void *x, int64_t ldx, const void *resi
         return fail(MOE_ERR_ARG, "%s: weight type %d: need fp32 or the rows' type", fn, w_dtype);
     if ((!q) != (!scale)) return fail(MOE_ERR_ARG, "%s: q and scale go together", fn);
     if (residual && !sum) return fail(MOE_ERR_ARG, "%s: a residual needs the sum's output", fn);
-    if (S < 0 || M < 1 || M > NORM_MAX_M) return fail(MOE_ERR_SHAPE, "%s: need S >= 0, 1 <= M <= %d (S=%d M=%d)", fn, NORM_MAX_M, S, M);
+    if (S < 0 || S > DIM_MAX || M < 1 || M > NORM_MAX_M)
+        return fail(MOE_ERR_SHAPE, "%s: need 0 <= S <= %d, 1 <= M <= %d (S=%d M=%d)", fn, DIM_MAX, NORM_MAX_M, S, M);
     if (S > 1 && (ldx < M || (residual && ldr < M) || (y && ldy < M) || (sum && lds < M)))
         return fail(MOE_ERR_SHAPE, "%s: row strides must be >= M", fn);
     if (q && ((M & 15) || (ldq & 7) || ldq < M || ld_scale < (M + QB - 1) / QB))
@@ -448,7 +449,8 @@ extern "C" int moe_add_rms_norm_bwd(const void *dy, int64_t lddy, const void *ds
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
     if (w_dtype != MOE_WG_F32 && w_dtype != (dtype == MOE_DTYPE_BF16 ? MOE_WG_BF16 : MOE_WG_F16))
         return fail(MOE_ERR_ARG, "%s: weight type %d: need fp32 or the rows' type", fn, w_dtype);
-    if (S < 1 || M < 1 || M > NORM_MAX_M) return fail(MOE_ERR_SHAPE, "%s: need S >= 1, 1 <= M <= %d (S=%d M=%d)", fn, NORM_MAX_M, S, M);
+    if (S < 1 || S > DIM_MAX || M < 1 || M > NORM_MAX_M)
+        return fail(MOE_ERR_SHAPE, "%s: need 1 <= S <= %d, 1 <= M <= %d (S=%d M=%d)", fn, DIM_MAX, NORM_MAX_M, S, M);
     if (S > 1 && ((dy && lddy < M) || (dsum && ldds < M) || lds < M || lddx < M)) return fail(MOE_ERR_SHAPE, "%s: row strides must be >= M", fn);
     if (!even2(dy) || !even2(dsum) || !even2(sum) || !even2(dx) || !even2(weight) || !even2(dweight) ||
         (w_dtype == MOE_WG_F32 && ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(dweight)) & 3)) ||
@@ -491,6 +493,7 @@ extern "C" int moe_quantize_rows_fp8(const void *x, int64_t ldx, int S, int M, v
     if (!x || !q || !scale) return fail(MOE_ERR_ARG, "%s: null pointer", fn);
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
     if (S < 0 || M < 16 || (M & 15)) return fail(MOE_ERR_SHAPE, "%s: need S >= 0, M >= 16, M %% 16 == 0 (S=%d M=%d)", fn, S, M);
+    if (S > DIM_MAX || M > DIM_MAX) return fail(MOE_ERR_SHAPE, "%s: S=%d, M=%d: at most %d", fn, S, M, DIM_MAX);
     if ((S > 1 && ldx < M) || ldq < M || (ldq & 7) || ld_scale < (M + QB - 1) / QB)
         return fail(MOE_ERR_SHAPE, "%s: row strides too small (or ldq %% 8 != 0)", fn);
     if (!even2(x) || (reinterpret_cast<uintptr_t>(q) & 7)) return fail(MOE_ERR_ALIGN, "%s: x must be 2-byte, q 8-byte aligned", fn);
@@ -512,6 +515,7 @@ extern "C" int moe_quantize_blocks_fp8(const void *w, int batch, int n, int k, v
     if (!w || !q || !scale) return fail(MOE_ERR_ARG, "%s: null pointer", fn);
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
     if (batch < 1 || n < 1 || k < 16 || (k & 15)) return fail(MOE_ERR_SHAPE, "%s: need batch >= 1, n >= 1, k %% 16 == 0 (%d, %d, %d)", fn, batch, n, k);
+    if (n > DIM_MAX || k > DIM_MAX) return fail(MOE_ERR_SHAPE, "%s: n=%d, k=%d: at most %d", fn, n, k, DIM_MAX);
     if (!aligned16(w) || (reinterpret_cast<uintptr_t>(q) & 7)) return fail(MOE_ERR_ALIGN, "%s: w must be 16-byte, q 8-byte aligned", fn);
     const long long g = (long long)batch * ((n + QB - 1) / QB) * ((k + QB - 1) / QB);
     if (!grid_fits(g, 256)) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);
@@ -527,6 +531,7 @@ extern "C" int moe_transpose_blocks_fp8(const void *w, const void *scale, int ba
     const char *fn = "moe_transpose_blocks_fp8";
     if (!w || !scale || !wt || !scale_t) return fail(MOE_ERR_ARG, "%s: null pointer", fn);
     if (batch < 1 || n < 16 || (n & 15) || k < 16 || (k & 15)) return fail(MOE_ERR_SHAPE, "%s: need n %% 16 == 0 and k %% 16 == 0 (%d, %d, %d)", fn, batch, n, k);
+    if (n > DIM_MAX || k > DIM_MAX) return fail(MOE_ERR_SHAPE, "%s: n=%d, k=%d: at most %d", fn, n, k, DIM_MAX);
     if (!aligned16(w) || !aligned16(wt)) return fail(MOE_ERR_ALIGN, "%s: weights must be 16-byte aligned", fn);
     const long long g = (long long)batch * ((n + 63) / 64) * ((k + 63) / 64);
     if (!grid_fits(g, 256)) return fail(MOE_ERR_SHAPE, "%s: too many blocks", fn);

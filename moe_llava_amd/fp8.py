@@ -26,7 +26,7 @@ BLOCK = 128
 E4M3 = torch.float8_e4m3fn
 E8M0 = torch.float8_e8m0fnu
 MAX_K = 65536            # columns of a product's operands
-MAX_ROWS = 2 ** 31 - 1   # row counts and matrix dimensions are 32-bit in the library
+MAX_ROWS = 2 ** 31 - 512  # row counts and matrix dimensions: rounded up to a tile they stay within the library's 32 bits
 _ACTS = {"swiglu": ops.ACT_SWIGLU, "gelu_new": ops.ACT_GELU_NEW, ops.ACT_SWIGLU: ops.ACT_SWIGLU,
          ops.ACT_GELU_NEW: ops.ACT_GELU_NEW}
 
@@ -73,8 +73,8 @@ def _half_rows(x: Tensor, name: str) -> Tensor:
         raise ValueError(f"{name}: expected at least one dimension")
     if d != 2:
         x = x.reshape(-1, x.shape[-1]) if x.numel() else x.reshape(x.shape[:-1].numel(), x.shape[-1])
-    if x.shape[0] > MAX_ROWS:
-        raise ValueError(f"{name}: {x.shape[0]} rows: at most {MAX_ROWS}")
+    if x.shape[0] > MAX_ROWS or x.shape[1] > MAX_ROWS:
+        raise ValueError(f"{name}: {tuple(x.shape)}: rows and columns of at most {MAX_ROWS}")
     if d == 2 and x.is_contiguous():
         return x
     if x.shape[1] > 1 and x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
@@ -134,6 +134,8 @@ def _check_weight(w: Tensor, ws: Tensor, name: str, E: int, N: Optional[int], pa
     n //= parts
     if K % 16 or not 16 <= K <= MAX_K:
         raise ValueError(f"{name}: K={K} must be a multiple of 16 and at most {MAX_K}")
+    if n > MAX_ROWS:
+        raise ValueError(f"{name}: N={n}: at most {MAX_ROWS}")
     if sc[-2] != parts * ((n + 127) // BLOCK) or sc[-1] != (K + 127) // BLOCK or (E and (sh[0] != E or sc[0] != E)) \
             or ws.device != w.device:
         raise ValueError(f"{name}_scale: {tuple(sc)} on {ws.device} does not match {name} {tuple(sh)} on {w.device}")
