@@ -192,16 +192,22 @@ class StreamOrder:
                 t.record_stream(st)           # freed memory is not handed out again before this stream is done with it
 
 
-_SPLITK_WS = {}      # (device index, stream pointer) -> 64 MiB workspace of the split-K tail
+class _Workspaces(threading.local):
+    def __init__(self):
+        self.kept = {}   # (device index, stream pointer) -> 64 MiB workspace of the split-K tail
+
+
+_SPLITK_WS = _Workspaces()
 _SPLITK_BYTES = None
 
 
 def _splitk_ws(t: Tensor, st: int):
     """(pointer, bytes, owner) of the split-K workspace of the grouped GEMM launches on stream ``st`` of ``t``'s device
-    (include/moe_gfx950.h: moe_splitk_workspace_bytes).  One buffer per (device, stream), allocated on first use and kept:
-    launches on one stream are ordered, launches on different streams (the chunks of the expert-parallel exchange
-    alternate between two) must not share it.  Launches that are captured get one from the graph's memory, as graphs
-    captured on one stream may be replayed on several; the caller holds ``owner`` until its launches are out.
+    (include/moe_gfx950.h: moe_splitk_workspace_bytes).  One buffer per (device, stream) and thread, allocated on first use
+    and kept: launches of one thread on one stream are ordered, launches on different streams (the chunks of the
+    expert-parallel exchange alternate between two) must not share it, and neither must threads on one stream, where another
+    call's products can come between a call's products and its fix-up.  Launches that are captured get one from the graph's
+    memory, as graphs captured on one stream may be replayed on several; the caller holds ``owner`` until its launches are out.
     ``MOE_SPLITK=0`` in the environment: no workspace, tiles stay whole."""
     global _SPLITK_BYTES
     if _SPLITK_BYTES is None:
@@ -214,10 +220,10 @@ def _splitk_ws(t: Tensor, st: int):
         ws = torch.empty((_SPLITK_BYTES,), dtype=torch.uint8, device=t.device)
         return ws.data_ptr(), _SPLITK_BYTES, ws
     key = (t.device.index, st)
-    ws = _SPLITK_WS.get(key)
+    kept = _SPLITK_WS.kept
+    ws = kept.get(key)
     if ws is None:
-        ws = torch.empty((_SPLITK_BYTES,), dtype=torch.uint8, device=t.device)
-        _SPLITK_WS[key] = ws
+        ws = kept[key] = torch.empty((_SPLITK_BYTES,), dtype=torch.uint8, device=t.device)
     return ws.data_ptr(), _SPLITK_BYTES, ws
 
 

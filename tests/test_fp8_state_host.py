@@ -261,14 +261,14 @@ def test_a_decode_step_runs_on_its_device(monkeypatch, eight):
 def test_captured_launches_share_no_splitk_workspace(monkeypatch):
     from types import SimpleNamespace
     monkeypatch.setattr(ops, "_SPLITK_BYTES", 4096)
-    monkeypatch.setattr(ops, "_SPLITK_WS", {})
+    monkeypatch.setattr(ops, "_SPLITK_WS", ops._Workspaces())
     t = SimpleNamespace(is_cuda=True, device=CPU)
     eager = ops._splitk_ws(t, 7)
     assert ops._splitk_ws(t, 7)[0] == eager[0] != ops._splitk_ws(t, 8)[0]
     monkeypatch.setattr(ops, "_capturing", lambda dev: True)
     held = [ops._splitk_ws(t, 7) for _ in range(2)]
     assert len({eager[0], held[0][0], held[1][0]}) == 3 and all(h[2].data_ptr() == h[0] for h in held)
-    assert len(ops._SPLITK_WS) == 2
+    assert len(ops._SPLITK_WS.kept) == 2
 
 
 def test_a_copy_of_the_layer_has_no_plans():
@@ -353,3 +353,12 @@ def test_threads_on_one_stream_have_plans_of_their_own(monkeypatch, made, eight)
     layer._decode_step(x, x, 1)
     _threads(2, lambda i: (layer._decode_step(x, x, 1), layer._decode_step(x, x, 1)))
     assert len(seen) == 5 and len(set(map(id, seen))) == 3
+
+
+def test_threads_on_one_stream_share_no_splitk_workspace(monkeypatch):
+    from types import SimpleNamespace
+    monkeypatch.setattr(ops, "_SPLITK_BYTES", 4096)
+    t = SimpleNamespace(is_cuda=True, device=CPU)
+    mine = ops._splitk_ws(t, 7)
+    held = _threads(3, lambda i: (ops._splitk_ws(t, 7), ops._splitk_ws(t, 7)))
+    assert all(a[0] == b[0] for a, b in held) and len({mine[0]} | {a[0] for a, _ in held}) == 4
